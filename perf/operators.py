@@ -515,9 +515,18 @@ def plain_pages(s):
 # --------------------------------------------------------------------------------------------------------------------
 # The framework's operators
 # --------------------------------------------------------------------------------------------------------------------
+def builders():
+    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pytorchsim-triton-backend_b200")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+    from pytorchsim_triton_compiler.codegen import build
+    return build
+
+
 def graph(s, key, steps):
     """Runs the launch graph of `steps` [(descriptor, names of its buffers)], built once over a state's buffers."""
     if key not in s:
+        builders()
         from pytorchsim_triton_compiler.codegen import descriptors as D
         from pytorchsim_triton_compiler.runtime.graph import Graph
         g = Graph("cuda:%d" % torch.cuda.current_device())
@@ -527,14 +536,6 @@ def graph(s, key, steps):
             g.add("step%d" % i, D.to_bytes(desc), names)
         s[key] = g
     s[key].run()
-
-
-def builders():
-    root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "pytorchsim-triton-backend_b200")
-    if root not in sys.path:
-        sys.path.insert(0, root)
-    from pytorchsim_triton_compiler.codegen import build
-    return build
 
 
 def own_prompt(s):
