@@ -59,6 +59,11 @@ extern "C" {
 #define PTSIM_KIND_GATHER_SUM 14   /* out[r, :] = sum over k of w(r, k) * table[t(r, k), :] (the MoE combine) */
 #define PTSIM_KIND_INT_TABLE 15    /* an int64 program over [rows, cols] stored per element, summed or scanned along a row */
 #define PTSIM_KIND_ROW_SUM 16      /* out[r] = fp32 sum of row r (the MoE layer's per-token weight sums) */
+#define PTSIM_KIND_ATTN_PACKED 17  /* causal GQA attention of packed prompts of different lengths */
+#define PTSIM_KIND_KV4_STORE 18    /* keys and values quantised to 4 bits into the pages of a cache */
+#define PTSIM_KIND_KV4_LOAD 19     /* cached keys and values back as dense rows */
+#define PTSIM_KIND_ATTN_KV4 20     /* one-token GQA attention per slot over its 4-bit cached keys and values */
+#define PTSIM_KIND_PAGES 21        /* page bookkeeping of a cache: grow, fork, copy, free, compact */
 
 /* Element types of tensor arguments (kernel.json dtype names, contract/kernel_object.py:43-56). */
 #define PTSIM_DT_F32 0
@@ -303,6 +308,76 @@ typedef struct ptsim_itab_params {
   ptsim_iinsn code[PTSIM_MAX_ICODE];
 } ptsim_itab_params;
 
+/* ATTN_PACKED: sequence s holds query rows cuq[s] .. cuq[s + 1] and key rows cuk[s] .. cuk[s + 1] (int32 tables of
+ * seqs + 1 entries, ascending, inside the tokens; cuq_arg and cuk_arg may be one argument).  With ql and kl rows,
+ * query i sees keys j <= i + kl - ql (the ends are aligned); o = sum_j softmax_j(scale q.k_j) v_j, and a query that sees
+ * no key gives zeros.  Keys a query does not see never reach its result, whatever they hold.  Rows of o outside every
+ * sequence keep their values.  Element (token t, head h, d) of x lies at x_off + t x_row + h x_head + d of argument
+ * x_arg (q, k, v may be parts of one argument); offsets and strides are multiples of 8 elements.  A table that
+ * descends or leaves the tokens records PTSIM_E_OOB and its sequence is skipped.  bf16 or fp16 throughout; dim 64 or
+ * 128; scale > 0, scores scale q.k below 2^30; at most PTSIM_PACKED_SEQS sequences.  One partition unit. */
+#define PTSIM_PACKED_SEQS 4096
+typedef struct ptsim_pattn_params {
+  int64_t q_tokens, k_tokens, seqs, hq, hkv, dim;
+  int64_t q_off, q_row, q_head, k_off, k_row, k_head, v_off, v_row, v_head, o_off, o_row, o_head;
+  int32_t q_arg, k_arg, v_arg, o_arg, cuq_arg, cuk_arg;
+  float scale, pad0;
+} ptsim_pattn_params;
+
+/* The 4-bit paged cache.  pool (uint8): layers x pages x hkv records; slot s holds lens[s] tokens (int32 [slots]),
+ * token t in page table[s][t / page_size] (int32 [slots][max_pages]).  A record is one page of one KV head: blocks of
+ * b = min(page_size, 32) tokens, each [K codes: b rows of dim / 2 bytes][V codes: the same][K parameters: b rows of
+ * dim / group pairs (scale, minimum) of the cache's 16-bit type][V parameters], PTSIM_KV4_PAGE_BYTES per page.  A group of
+ * `group` values along the head dimension holds code = clamp(rint((x - minimum) / scale), 0, 15) with
+ * scale = T((max - min) / 15) (code 0 where scale is 0) and stands for scale * code + minimum; a group with a
+ * non-finite value reads back as NaN.  Codes are placed as the attention's tensor-core operands take them:
+ *   K row of token t, row t of the block: 32-bit word (d % 32 / 8) * (dim / 32) + d / 32, nibble (d % 8) / 2 + 4 (d % 2);
+ *   V row of token t, row r = (t & ~7) | (t & 1) << 2 | (t >> 1 & 3): word (c * (dim / 64) + d / 64) with
+ *   c = d % 32 / 4, c ^ 4 for dim 128 where r & 2, nibble d % 4 + 4 (d % 64 / 32).
+ *
+ * KV4_STORE: token rows cu[s] .. cu[s + 1] of a (keys) and b (values) become the last tokens of slot s, which holds
+ * lens[s] tokens with them (its pages are in the table already).  KV4_LOAD: the reverse, the last cu[s + 1] - cu[s]
+ * tokens of slot s into rows of a and b, scale * code + minimum in fp32 rounded to their type; rows of no slot are
+ * left alone.  ATTN_KV4: a = q, b = o,
+ * rows of one token per slot: query head h of slot s attends over the lens[s] cached tokens of KV head h / (hq / hkv); a
+ * slot of length 0 gives zeros.  Element (row t, head h, d) of x lies at x_off + t x_row + h x_head + d, offsets and
+ * strides multiples of 8 elements.  A token outside the table's row, or a page outside the pool, records PTSIM_E_OOB
+ * and is not written, reads as zeros, is not attended to.  One partition unit. */
+#define PTSIM_KV4_PAGE_BYTES(hkv, page_size, dim, group) ((hkv) * (page_size) * ((dim) + 8 * ((dim) / (group))))
+#define PTSIM_KV4_SLOTS 4096
+typedef struct ptsim_kv4_params {
+  int64_t tokens, slots, hq, hkv, dim, group;           /* tokens: rows of a and b (STORE, LOAD); hq: ATTN_KV4 */
+  int64_t pages, page_size, max_pages, layers, layer;   /* page_size 16, 32, 64 or 128; dim 64 or 128; group 32, 64, 128 */
+  int64_t a_off, a_row, a_head, b_off, b_row, b_head;
+  int32_t a_arg, b_arg, cu_arg, lens_arg, table_arg, pool_arg;   /* cu_arg -1: ATTN_KV4 */
+  float scale, pad0;
+} ptsim_kv4_params;
+
+/* PAGES: the bookkeeping of such a cache (any pool of layers x pages x page_bytes, page_bytes a multiple of 16).  refs
+ * (int32 [pages]) counts the slots that hold a page; a page with 0 is free.  A launch takes the slots ids[n] in order:
+ *   GROW     aux[i] >= 0 tokens more for slot ids[i]: the pages it lacks are the lowest free ones, counted once;
+ *   FORK     slot aux[i] (empty) becomes slot ids[i]'s copy: full pages are shared, a partial last page is copied to the
+ *            lowest free page in every layer;   COPY  the same with every page copied;
+ *   FREE     the pages of slot ids[i] lose one count, its table entries become -1, its length 0 (a slot listed twice
+ *            is freed once);
+ *   COMPACT  (n = 0) with L pages in use, the k-th used page at or past L moves to the k-th free page below L, in every
+ *            layer, and the tables follow; used pages are then 0 .. L - 1.
+ * Refused on the device, nothing changed (GROW, FORK, COPY): a slot outside the table or of an impossible length
+ * (PTSIM_E_OOB); a negative aux of GROW, a slot listed twice in GROW, a target listed twice, not empty or also a source
+ * (PTSIM_E_ARGS); a slot whose row cannot hold its pages or too few free pages (PTSIM_E_RESOURCE).  FREE and COMPACT record
+ * such a slot (PTSIM_E_OOB) and pass over it.  A held table entry outside the pool is recorded (PTSIM_E_OOB) and not
+ * counted, copied or moved.  One partition unit. */
+#define PTSIM_PAGES_GROW 1
+#define PTSIM_PAGES_FORK 2
+#define PTSIM_PAGES_COPY 3
+#define PTSIM_PAGES_FREE 4
+#define PTSIM_PAGES_COMPACT 5
+#define PTSIM_PAGES_IDS 1024
+typedef struct ptsim_pages_params {
+  int64_t n, slots, pages, page_size, max_pages, layers, page_bytes;
+  int32_t op, ids_arg, aux_arg, table_arg, lens_arg, refs_arg, pool_arg, pad0;
+} ptsim_pages_params;
+
 typedef struct ptsim_reduce_params {
   int64_t numel;
   int32_t in_arg, out_arg, op, pad0;
@@ -334,6 +409,9 @@ typedef struct ptsim_desc {
     ptsim_ggemm_params ggemm;
     ptsim_gsum_params gsum;
     ptsim_itab_params itab;
+    ptsim_pattn_params pattn;
+    ptsim_kv4_params kv4;
+    ptsim_pages_params pages;
   } p;
 } ptsim_desc;
 

@@ -15,6 +15,9 @@
 #include "moe.cuh"
 #include "itable.cuh"
 #include "collective.cuh"
+#include "packed.cuh"
+#include "kv4.cuh"
+#include "pages.cuh"
 
 namespace ptsim {
 
@@ -89,6 +92,124 @@ static int check_vprog(const ptsim_desc &d, const ptsim_vprog &v, const char *wh
         (c.op == PTSIM_OP_LOAD ? c.a >= v.nload : c.a >= 8))
       return fail(PTSIM_E_DESC, "%s instruction %d", what, i);
   }
+  return PTSIM_OK;
+}
+
+// The last element a serving tensor's rows reach: `rows` tokens of `heads` heads of `dim` values; offsets and strides keep every
+// (token, head) row on a 16-byte boundary, which TMA and the wide loads need.
+static int check_rows(const ptsim_desc &d, int arg, int64_t off, int64_t row, int64_t head, int64_t rows, int64_t heads, int64_t dim,
+                      const char *what) {
+  int rc = check_arg(d, arg, what);
+  if (rc) return rc;
+  if (off < 0 || row < 0 || head < 0 || row >= (int64_t(1) << 38) || head >= (int64_t(1) << 38))
+    return fail(PTSIM_E_DESC, "%s: offset %lld, strides %lld and %lld", what, (long long)off, (long long)row, (long long)head);
+  if (off % 8 != 0 || row % 8 != 0 || head % 8 != 0)
+    return fail(PTSIM_E_UNSUPPORTED, "%s: its offset and strides must be multiples of 8 elements", what);
+  if (rows > 0 && off + (rows - 1) * row + (heads - 1) * head + dim > d.arg_numel[arg])
+    return fail(PTSIM_E_OOB, "%s extends past its tensor", what);
+  return PTSIM_OK;
+}
+
+// An int32 table argument of at least n entries.
+static int check_ints(const ptsim_desc &d, int arg, int64_t n, const char *what) {
+  int rc = check_arg(d, arg, what);
+  if (rc) return rc;
+  if (d.arg_dtype[arg] != PTSIM_DT_I32) return fail(PTSIM_E_UNSUPPORTED, "%s must be int32", what);
+  if (n > d.arg_numel[arg]) return fail(PTSIM_E_OOB, "%s holds %lld entries, %lld are needed", what, (long long)d.arg_numel[arg], (long long)n);
+  return PTSIM_OK;
+}
+
+static int check_packed(const ptsim_desc &d) {
+  const ptsim_pattn_params &a = d.p.pattn;
+  const int64_t most = int64_t(1) << 30;
+  if (a.q_tokens < 0 || a.k_tokens < 0 || a.seqs < 0 || a.q_tokens > most || a.k_tokens > most || a.hkv < 1 || a.hq < 1 || a.hq > 65535 ||
+      a.hq % a.hkv != 0)
+    return fail(PTSIM_E_DESC, "packed attention of %lld and %lld tokens with %lld query heads over %lld KV heads", (long long)a.q_tokens,
+                (long long)a.k_tokens, (long long)a.hq, (long long)a.hkv);
+  if (a.dim != 64 && a.dim != 128) return fail(PTSIM_E_UNSUPPORTED, "packed attention with head dim %lld (runs 64 and 128)", (long long)a.dim);
+  if (a.seqs > PTSIM_PACKED_SEQS) return fail(PTSIM_E_UNSUPPORTED, "packed attention of %lld sequences (runs %d)", (long long)a.seqs, PTSIM_PACKED_SEQS);
+  if (!(a.scale > 0.f && a.scale < INFINITY)) return fail(PTSIM_E_UNSUPPORTED, "packed attention with scale %g", a.scale);
+  int rc;
+  if ((rc = check_rows(d, a.q_arg, a.q_off, a.q_row, a.q_head, a.q_tokens, a.hq, a.dim, "q")) ||
+      (rc = check_rows(d, a.k_arg, a.k_off, a.k_row, a.k_head, a.k_tokens, a.hkv, a.dim, "k")) ||
+      (rc = check_rows(d, a.v_arg, a.v_off, a.v_row, a.v_head, a.k_tokens, a.hkv, a.dim, "v")) ||
+      (rc = check_rows(d, a.o_arg, a.o_off, a.o_row, a.o_head, a.q_tokens, a.hq, a.dim, "o")) ||
+      (rc = check_ints(d, a.cuq_arg, a.seqs + 1, "the table of query rows")) ||
+      (rc = check_ints(d, a.cuk_arg, a.seqs + 1, "the table of key rows")))
+    return rc;
+  const int dt = d.arg_dtype[a.q_arg];
+  if ((dt != PTSIM_DT_BF16 && dt != PTSIM_DT_F16) || d.arg_dtype[a.k_arg] != dt || d.arg_dtype[a.v_arg] != dt || d.arg_dtype[a.o_arg] != dt)
+    return fail(PTSIM_E_UNSUPPORTED, "packed attention runs bf16 or fp16, one type for q, k, v and o");
+  if (a.o_arg == a.q_arg || a.o_arg == a.k_arg || a.o_arg == a.v_arg)
+    return fail(PTSIM_E_DESC, "packed attention writes an argument of its own");
+  return PTSIM_OK;
+}
+
+// A cache's sizes: slots x max_pages tables, layers x pages of page_bytes.
+static int check_cache(const ptsim_desc &d, int64_t slots, int64_t pages, int64_t page_size, int64_t max_pages, int64_t layers,
+                       int64_t page_bytes, int table_arg, int lens_arg, int pool_arg) {
+  const int64_t most = int64_t(1) << 30;
+  if (slots < 0 || pages < 0 || max_pages < 0 || layers < 1 || page_size < 1 || page_bytes < 16 || page_bytes % 16 != 0 || slots > most ||
+      pages > most || layers > 65536 || page_bytes > most || max_pages > most / page_size)
+    return fail(PTSIM_E_DESC, "a cache of %lld slots of %lld pages, %lld x %lld pages of %lld tokens and %lld bytes", (long long)slots,
+                (long long)max_pages, (long long)layers, (long long)pages, (long long)page_size, (long long)page_bytes);
+  int rc;
+  if ((rc = check_ints(d, table_arg, slots * max_pages, "the page table")) || (rc = check_ints(d, lens_arg, slots, "the lengths"))) return rc;
+  if (pool_arg < 0) return PTSIM_OK;
+  if ((rc = check_arg(d, pool_arg, "pool"))) return rc;
+  if (d.arg_dtype[pool_arg] != PTSIM_DT_U8) return fail(PTSIM_E_UNSUPPORTED, "the pool must be uint8");
+  if (pages > 0 && d.arg_numel[pool_arg] / page_bytes / pages < layers)
+    return fail(PTSIM_E_OOB, "the pool holds fewer than %lld x %lld pages of %lld bytes", (long long)layers, (long long)pages, (long long)page_bytes);
+  return PTSIM_OK;
+}
+
+static int check_kv4(const ptsim_desc &d) {
+  const ptsim_kv4_params &q = d.p.kv4;
+  const bool attn = d.kind == PTSIM_KIND_ATTN_KV4;
+  if ((q.dim != 64 && q.dim != 128) || (q.group != 32 && q.group != 64 && q.group != 128) || q.group > q.dim ||
+      (q.page_size != 16 && q.page_size != 32 && q.page_size != 64 && q.page_size != 128))
+    return fail(PTSIM_E_UNSUPPORTED, "a 4-bit cache of head dim %lld, groups of %lld, pages of %lld tokens", (long long)q.dim, (long long)q.group,
+                (long long)q.page_size);
+  if (q.hkv < 1 || q.hkv > 4096 || q.layer < 0 || q.layer >= q.layers || q.tokens < 0 || q.tokens > (int64_t(1) << 30))
+    return fail(PTSIM_E_DESC, "a 4-bit cache of %lld KV heads, layer %lld of %lld, %lld tokens", (long long)q.hkv, (long long)q.layer,
+                (long long)q.layers, (long long)q.tokens);
+  if (q.slots > PTSIM_KV4_SLOTS) return fail(PTSIM_E_UNSUPPORTED, "a 4-bit cache of %lld slots (runs %d)", (long long)q.slots, PTSIM_KV4_SLOTS);
+  int rc = check_cache(d, q.slots, q.pages, q.page_size, q.max_pages, q.layers,
+                       PTSIM_KV4_PAGE_BYTES(q.hkv, q.page_size, q.dim, q.group), q.table_arg, q.lens_arg, q.pool_arg);
+  if (rc) return rc;
+  if (q.pool_arg < 0) return fail(PTSIM_E_DESC, "a 4-bit cache without a pool");
+  if (attn) {
+    if (q.hq < 1 || q.hq % q.hkv != 0 || q.hq > 65536)
+      return fail(PTSIM_E_DESC, "4-bit cache attention with %lld query heads over %lld KV heads", (long long)q.hq, (long long)q.hkv);
+    if (!(q.scale > 0.f && q.scale < INFINITY)) return fail(PTSIM_E_UNSUPPORTED, "4-bit cache attention with scale %g", q.scale);
+    if (q.slots * q.hkv * ceil_div(q.hq / q.hkv, 16) * ceil_div(q.max_pages * q.page_size, 32) >= (int64_t(1) << 31))
+      return fail(PTSIM_E_UNSUPPORTED, "4-bit cache attention over more than 2^31 tiles of 32 keys");
+  } else if ((rc = check_ints(d, q.cu_arg, q.slots + 1, "the table of token rows"))) {
+    return rc;
+  }
+  const int64_t rows = attn ? q.slots : q.tokens, heads = attn ? q.hq : q.hkv;
+  if ((rc = check_rows(d, q.a_arg, q.a_off, q.a_row, q.a_head, rows, heads, q.dim, attn ? "q" : "k")) ||
+      (rc = check_rows(d, q.b_arg, q.b_off, q.b_row, q.b_head, rows, heads, q.dim, attn ? "o" : "v")))
+    return rc;
+  const int dt = d.arg_dtype[q.a_arg];
+  if ((dt != PTSIM_DT_BF16 && dt != PTSIM_DT_F16) || d.arg_dtype[q.b_arg] != dt)
+    return fail(PTSIM_E_UNSUPPORTED, "a 4-bit cache stands for bf16 or fp16 values, one type throughout");
+  if (d.kind != PTSIM_KIND_KV4_STORE && q.a_arg == q.b_arg) return fail(PTSIM_E_DESC, "the 4-bit cache's output is an argument of its own");
+  return PTSIM_OK;
+}
+
+static int check_pages(const ptsim_desc &d) {
+  const ptsim_pages_params &q = d.p.pages;
+  if (q.op < PTSIM_PAGES_GROW || q.op > PTSIM_PAGES_COMPACT) return fail(PTSIM_E_DESC, "page operation %d", q.op);
+  if (q.n < 0 || (q.op == PTSIM_PAGES_COMPACT && q.n != 0)) return fail(PTSIM_E_DESC, "page operation over %lld slots", (long long)q.n);
+  if (q.n > PTSIM_PAGES_IDS) return fail(PTSIM_E_UNSUPPORTED, "page operation over %lld slots (runs %d)", (long long)q.n, PTSIM_PAGES_IDS);
+  const bool moves = q.op != PTSIM_PAGES_GROW && q.op != PTSIM_PAGES_FREE;
+  if (moves && q.pool_arg < 0) return fail(PTSIM_E_DESC, "a page operation that moves pages has no pool");
+  int rc = check_cache(d, q.slots, q.pages, q.page_size, q.max_pages, q.layers, q.page_bytes, q.table_arg, q.lens_arg, moves ? q.pool_arg : -1);
+  if (rc || (rc = check_ints(d, q.refs_arg, q.pages, "the page counts"))) return rc;
+  if (q.op != PTSIM_PAGES_COMPACT && (rc = check_ints(d, q.ids_arg, q.n, "the listed slots"))) return rc;
+  if (q.op < PTSIM_PAGES_FREE && (rc = check_ints(d, q.aux_arg, q.n, "the second list"))) return rc;
+  if (q.slots == 0 && q.n > 0) return fail(PTSIM_E_DESC, "a page operation on a cache without slots");
   return PTSIM_OK;
 }
 
@@ -331,6 +452,14 @@ static int check_desc(const void *p, size_t bytes) {
         return fail(PTSIM_E_OOB, "reduction past its tensors");
       break;
     }
+    case PTSIM_KIND_ATTN_PACKED:
+    case PTSIM_KIND_KV4_STORE:
+    case PTSIM_KIND_KV4_LOAD:
+    case PTSIM_KIND_ATTN_KV4:
+    case PTSIM_KIND_PAGES:
+      if ((rc = d.kind == PTSIM_KIND_ATTN_PACKED ? check_packed(d) : d.kind == PTSIM_KIND_PAGES ? check_pages(d) : check_kv4(d))) return rc;
+      if (d.units != 1 || d.unit_size != 1) return fail(PTSIM_E_DESC, "a serving launch is one unit");
+      break;
     default:
       return fail(PTSIM_E_DESC, "descriptor kind %u is not one this library runs", d.kind);
   }
@@ -474,6 +603,11 @@ static int launch_desc(const void *desc, size_t desc_bytes, void *const *dev_ptr
     case PTSIM_KIND_ATTN_PREFILL: return launch_attention(d, dev_ptrs, lo, hi, c);
     case PTSIM_KIND_REDUCE_ALL: return launch_reduce(d, dev_ptrs, lo, hi, workspace, workspace_bytes, c);
     case PTSIM_KIND_ATTN_DECODE: return launch_decode(d, dev_ptrs, lo, hi, workspace, workspace_bytes, c);
+    case PTSIM_KIND_ATTN_PACKED: return launch_packed(d, dev_ptrs, c);
+    case PTSIM_KIND_KV4_STORE:
+    case PTSIM_KIND_KV4_LOAD:
+    case PTSIM_KIND_ATTN_KV4: return launch_kv4(d, dev_ptrs, workspace, workspace_bytes, c);
+    case PTSIM_KIND_PAGES: return launch_pages(d, dev_ptrs, workspace, workspace_bytes, c);
   }
   return fail(PTSIM_E_DESC, "descriptor kind %u", d.kind);
 }
@@ -493,6 +627,8 @@ int64_t ptsim_workspace_size(const void *desc, size_t desc_bytes, int device) {
   if (d.kind == PTSIM_KIND_INT_TABLE && need < itab_workspace(d, sm_count)) need = itab_workspace(d, sm_count);
   if (d.kind == PTSIM_KIND_GEMM && need < gemv_workspace(d, sm_count)) need = gemv_workspace(d, sm_count);
   if (d.kind == PTSIM_KIND_SORT && need < sort_workspace(d)) need = sort_workspace(d);
+  if (d.kind == PTSIM_KIND_ATTN_KV4 && need < kv4_workspace(d, sm_count)) need = kv4_workspace(d, sm_count);
+  if (d.kind == PTSIM_KIND_PAGES && need < pages_workspace(d)) need = pages_workspace(d);
   return need;
 }
 

@@ -37,4 +37,22 @@ static int make_tmap_2d(CUtensorMap *m, const void *base, uint64_t cols, uint64_
   return PTSIM_OK;
 }
 
+// 3-D map of 16-bit elements [heads][rows][cols] with any (16-byte multiple) row and head strides, box {box_cols,
+// box_rows, 1}, 128-byte swizzle, zero fill outside the tensor.
+static int make_tmap_heads(CUtensorMap *m, const void *base, uint64_t cols, uint64_t rows, uint64_t heads, int64_t row_stride,
+                           int64_t head_stride, uint32_t box_cols, uint32_t box_rows) {
+  auto enc = get_encode_tiled();
+  if (enc == nullptr) return fail(PTSIM_E_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  if (reinterpret_cast<uintptr_t>(base) % 16 != 0) return fail(PTSIM_E_ARGS, "TMA base address not 16-byte aligned");
+  cuuint64_t dims[3] = {cols, rows, heads};
+  cuuint64_t strides[2] = {cuuint64_t(row_stride) * 2, cuuint64_t(head_stride) * 2};
+  cuuint32_t box[3] = {box_cols, box_rows, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(PTSIM_E_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
+  return PTSIM_OK;
+}
+
 }  // namespace ptsim

@@ -101,6 +101,152 @@ def attention_decode(hkv, group, seq, dim=128, scale=None, bkv=None, gp=16):
     return d
 
 
+def _place(params, name, arg, off, row, head):
+    """Where tensor `name` of a serving descriptor lies: its argument, and the offset of element (row t, head h, d)."""
+    for k, v in (("arg", arg), ("off", off), ("row", row), ("head", head)):
+        setattr(params, f"{name}_{k}", v)
+
+
+def attention_packed(tokens, seqs, hq, hkv, dim=128, scale=None, dtype="bfloat16", k_tokens=None, fused=False,
+                     head_major=False):
+    """Causal GQA attention of `seqs` prompts packed back to back: sequence s is rows cu[s] .. cu[s + 1] (int32
+    [seqs + 1]).  Arguments q [tokens, hq, dim], k, v [tokens, hkv, dim], cu, o [tokens, hq, dim]; with `k_tokens`,
+    keys of lengths of their own (a prefix cached earlier; the ends of queries and keys are aligned): q, k, v, cuq, cuk,
+    o; `fused`: one projection qkv [tokens, hq + 2 hkv, dim], cu, o; `head_major`: q, k, v, o are [heads, tokens, dim], as
+    qknorm_rope and attention keep them."""
+    import math
+    if fused and (head_major or k_tokens is not None):
+        raise ValueError("a fused projection holds one token's q, k and v together")
+    nk = tokens if k_tokens is None else k_tokens
+    cu = [("cu_ptr", "int32", seqs + 1)] if k_tokens is None else [("cuq_ptr", "int32", seqs + 1), ("cuk_ptr", "int32", seqs + 1)]
+    qkv = [("qkv_ptr", dtype, tokens * (hq + 2 * hkv) * dim)] if fused else \
+        [("q_ptr", dtype, tokens * hq * dim), ("k_ptr", dtype, nk * hkv * dim), ("v_ptr", dtype, nk * hkv * dim)]
+    specs = qkv + cu + [("o_ptr", dtype, tokens * hq * dim)]
+    d = D.new(D.ATTN_PACKED, _args(specs), (1, 1, 1), units=1, unit_size=1)
+    a = d.p.pattn
+    a.q_tokens, a.k_tokens, a.seqs, a.hq, a.hkv, a.dim = tokens, nk, seqs, hq, hkv, dim
+    a.scale = float(scale if scale is not None else 1.0 / math.sqrt(dim))
+    if fused:
+        row = (hq + 2 * hkv) * dim
+        for name, off in (("q", 0), ("k", hq * dim), ("v", (hq + hkv) * dim)):
+            _place(a, name, 0, off, row, dim)
+    else:
+        for i, (name, n, h) in enumerate((("q", tokens, hq), ("k", nk, hkv), ("v", nk, hkv))):
+            _place(a, name, i, 0, *((dim, n * dim) if head_major else (h * dim, dim)))
+    _place(a, "o", len(specs) - 1, 0, *((dim, tokens * dim) if head_major else (hq * dim, dim)))
+    a.cuq_arg, a.cuk_arg = len(qkv), len(specs) - 2
+    return d
+
+
+class kv4_cache:
+    """The shape of a 4-bit paged cache (include/ptsim_b200.h, ptsim_kv4_params): the pool's and the table's sizes that
+    the cache's launches share.  `dtype` is the type of the keys and values it stands for."""
+
+    def __init__(self, slots, max_pages, pages, hkv, dim=128, page_size=16, group=64, layers=1, dtype="bfloat16"):
+        if dim not in (64, 128) or page_size not in (16, 32, 64, 128) or group not in (32, 64, 128) or group > dim:
+            raise ValueError(f"a 4-bit cache of head dim {dim}, page size {page_size}, group {group}")
+        self.slots, self.max_pages, self.pages, self.hkv, self.dim = slots, max_pages, pages, hkv, dim
+        self.page_size, self.group, self.layers, self.dtype = page_size, group, layers, dtype
+        self.page_bytes = hkv * page_size * (dim + 8 * (dim // group))
+        self.pool_bytes = layers * pages * self.page_bytes
+
+    def books(self):
+        return [("lens_ptr", "int32", self.slots), ("table_ptr", "int32", self.slots * self.max_pages),
+                ("pool_ptr", "uint8", self.pool_bytes)]
+
+
+def _kv4(kind, cache, specs, layer, **fields):
+    d = D.new(kind, _args(specs), (1, 1, 1), units=1, unit_size=1)
+    q, i = d.p.kv4, {n: k for k, (n, _, _) in enumerate(specs)}
+    for n in ("slots", "hkv", "dim", "group", "pages", "page_size", "max_pages", "layers"):
+        setattr(q, n, getattr(cache, n))
+    q.layer = layer
+    for n, v in fields.items():
+        setattr(q, n, v)
+    q.lens_arg, q.table_arg, q.pool_arg, q.cu_arg = i["lens_ptr"], i["table_ptr"], i["pool_ptr"], i.get("cu_ptr", -1)
+    return d
+
+
+def kv4_store(cache, tokens, layer=0, fused_hq=None, head_major=False):
+    """New keys and values into a 4-bit cache: rows cu[s] .. cu[s + 1] become the last tokens of slot s, which holds lens[s]
+    tokens with them.  Arguments k, v [tokens, hkv, dim], cu (int32 [slots + 1]), lens, table, pool; `fused_hq`: one
+    projection qkv [tokens, fused_hq + 2 hkv, dim] in the place of k and v; `head_major`: k is [hkv, tokens, dim]."""
+    n = cache.hkv * cache.dim
+    if fused_hq is not None and head_major:
+        raise ValueError("a fused projection holds one token's q, k and v together")
+    kv = [("qkv_ptr", cache.dtype, tokens * (fused_hq * cache.dim + 2 * n))] if fused_hq is not None else \
+        [("k_ptr", cache.dtype, tokens * n), ("v_ptr", cache.dtype, tokens * n)]
+    d = _kv4(D.KV4_STORE, cache, kv + [("cu_ptr", "int32", cache.slots + 1)] + cache.books(), layer, tokens=tokens)
+    if fused_hq is not None:
+        row = fused_hq * cache.dim + 2 * n
+        _place(d.p.kv4, "a", 0, fused_hq * cache.dim, row, cache.dim)
+        _place(d.p.kv4, "b", 0, fused_hq * cache.dim + n, row, cache.dim)
+    else:
+        _place(d.p.kv4, "a", 0, 0, *((cache.dim, tokens * cache.dim) if head_major else (n, cache.dim)))
+        _place(d.p.kv4, "b", 1, 0, n, cache.dim)
+    return d
+
+
+def kv4_load(cache, tokens, layer=0):
+    """The last cu[s + 1] - cu[s] tokens of each slot back as rows cu[s] .. of dense k, v [tokens, hkv, dim]: arguments
+    cu, lens, table, pool, k, v."""
+    n = cache.hkv * cache.dim
+    d = _kv4(D.KV4_LOAD, cache, [("cu_ptr", "int32", cache.slots + 1)] + cache.books() +
+             [("k_ptr", cache.dtype, tokens * n), ("v_ptr", cache.dtype, tokens * n)], layer, tokens=tokens)
+    _place(d.p.kv4, "a", 4, 0, n, cache.dim)
+    _place(d.p.kv4, "b", 5, 0, n, cache.dim)
+    return d
+
+
+def attention_kv4(cache, hq, layer=0, scale=None, fused=False):
+    """One-token GQA attention of every slot over its lens[s] cached tokens: arguments q [slots, hq, dim], lens, table, pool,
+    o [slots, hq, dim]; `fused`: q is the first part of a projection qkv [slots, hq + 2 hkv, dim]."""
+    import math
+    row = (hq + 2 * cache.hkv) * cache.dim if fused else hq * cache.dim
+    specs = [("q_ptr", cache.dtype, cache.slots * row)] + cache.books() + [("o_ptr", cache.dtype, cache.slots * hq * cache.dim)]
+    d = _kv4(D.ATTN_KV4, cache, specs, layer, hq=hq)
+    d.p.kv4.scale = float(scale if scale is not None else 1.0 / math.sqrt(cache.dim))
+    _place(d.p.kv4, "a", 0, 0, row, cache.dim)
+    _place(d.p.kv4, "b", 4, 0, hq * cache.dim, cache.dim)
+    return d
+
+
+def _pages(op, cache, lists, pool):
+    specs = [(n, "int32", k) for n, k in lists] + [("table_ptr", "int32", cache.slots * cache.max_pages),
+                                                   ("lens_ptr", "int32", cache.slots), ("refs_ptr", "int32", cache.pages)]
+    if pool:
+        specs.append(("pool_ptr", "uint8", cache.pool_bytes))
+    d = D.new(D.PAGES, _args(specs), (1, 1, 1), units=1, unit_size=1)
+    q, m = d.p.pages, len(lists)
+    q.n = lists[0][1] if lists else 0
+    for n in ("slots", "pages", "page_size", "max_pages", "layers", "page_bytes"):
+        setattr(q, n, getattr(cache, n))
+    q.op, q.ids_arg, q.aux_arg = D.PAGES_OP[op], 0 if m > 0 else -1, 1 if m > 1 else -1
+    q.table_arg, q.lens_arg, q.refs_arg, q.pool_arg = m, m + 1, m + 2, m + 3 if pool else -1
+    return d
+
+
+def pages_grow(cache, n):
+    """Room for add[i] more tokens in slot ids[i]: arguments ids, add (int32 [n]), table, lens, refs."""
+    return _pages("grow", cache, [("ids_ptr", n), ("add_ptr", n)], False)
+
+
+def pages_fork(cache, n, deep=False):
+    """Empty slot dst[i] as a copy of slot src[i], sharing its full pages (`deep`: none): arguments src, dst (int32
+    [n]), table, lens, refs, pool."""
+    return _pages("copy" if deep else "fork", cache, [("src_ptr", n), ("dst_ptr", n)], True)
+
+
+def pages_free(cache, n):
+    """Slots ids[i] give their pages back: arguments ids (int32 [n]), table, lens, refs."""
+    return _pages("free", cache, [("ids_ptr", n)], False)
+
+
+def pages_compact(cache):
+    """Used pages moved to the front of the pool: arguments table, lens, refs, pool."""
+    return _pages("compact", cache, [], True)
+
+
 def gemv(N, K, b_kmajor=False, residual=False, out_dtype="bfloat16"):
     """The gemm_1x* program (Inductor's M = 1 matmul, a multiply-reduce): out[n] = sum_k a[k] * B[k, n]."""
     return gemm(1, N, K, residual=residual, b_kmajor=b_kmajor, out_dtype=out_dtype)

@@ -13,11 +13,13 @@ MAX_ARGS, MAX_MAPS, MAX_DIGITS, MAX_CODE, MAX_REGS = 16, 8, 4, 32, 8
 # Kinds (PTSIM_KIND_*).
 ELEMENTWISE, ROW_SOFTMAX, ROW_RMSNORM, QKNORM_ROPE, GEMM, ATTN_PREFILL, REDUCE_ALL, ATTN_DECODE = 1, 2, 3, 4, 5, 6, 7, 8
 ROW_DIVSUM, TOPK, SORT, GATHER_ROWS, GROUPED_GEMM, GATHER_SUM, INT_TABLE, ROW_SUM = 9, 10, 11, 12, 13, 14, 15, 16
+ATTN_PACKED, KV4_STORE, KV4_LOAD, ATTN_KV4, PAGES = 17, 18, 19, 20, 21
 KIND_NAME = {ELEMENTWISE: "elementwise", ROW_SOFTMAX: "row_softmax", ROW_RMSNORM: "row_rmsnorm",
              QKNORM_ROPE: "qknorm_rope", GEMM: "gemm", ATTN_PREFILL: "attn_prefill", REDUCE_ALL: "reduce_all",
              ATTN_DECODE: "attn_decode", ROW_DIVSUM: "row_divsum", TOPK: "topk", SORT: "sort",
              GATHER_ROWS: "gather_rows", GROUPED_GEMM: "grouped_gemm", GATHER_SUM: "gather_sum",
-             INT_TABLE: "int_table", ROW_SUM: "row_sum"}
+             INT_TABLE: "int_table", ROW_SUM: "row_sum", ATTN_PACKED: "attn_packed", KV4_STORE: "kv4_store",
+             KV4_LOAD: "kv4_load", ATTN_KV4: "attn_kv4", PAGES: "pages"}
 
 # Element types (PTSIM_DT_*), keyed by kernel.json dtype names (contract/kernel_object.py NP_DTYPE keys).
 DTYPE_CODE = {"float32": 0, "bfloat16": 1, "float16": 2, "int32": 3, "int64": 4, "int16": 5, "int8": 6,
@@ -153,10 +155,40 @@ class ItabParams(C.Structure):
                 ("maps", Map * ITAB_MAPS), ("out", ItabOut * ITAB_OUTS), ("code", IInsn * MAX_ICODE)]
 
 
+PACKED_SEQS, KV4_SLOTS, PAGES_IDS = 4096, 4096, 1024   # PTSIM_PACKED_SEQS, PTSIM_KV4_SLOTS, PTSIM_PAGES_IDS
+
+
+class PackedAttnParams(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("q_tokens", "k_tokens", "seqs", "hq", "hkv", "dim")] + \
+               [(f"{x}_{n}", C.c_int64) for x in "qkvo" for n in ("off", "row", "head")] + \
+               [(n, C.c_int32) for n in ("q_arg", "k_arg", "v_arg", "o_arg", "cuq_arg", "cuk_arg")] + \
+               [("scale", C.c_float), ("pad0", C.c_float)]
+
+
+class Kv4Params(C.Structure):
+    """ptsim_kv4_params: the 4-bit paged cache's store, load and attention."""
+    _fields_ = [(n, C.c_int64) for n in ("tokens", "slots", "hq", "hkv", "dim", "group", "pages", "page_size",
+                                         "max_pages", "layers", "layer")] + \
+               [(f"{x}_{n}", C.c_int64) for x in "ab" for n in ("off", "row", "head")] + \
+               [(n, C.c_int32) for n in ("a_arg", "b_arg", "cu_arg", "lens_arg", "table_arg", "pool_arg")] + \
+               [("scale", C.c_float), ("pad0", C.c_float)]
+
+
+PAGES_OP = {"grow": 1, "fork": 2, "copy": 3, "free": 4, "compact": 5}
+PAGES_OP_NAME = {v: k for k, v in PAGES_OP.items()}
+
+
+class PagesParams(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("n", "slots", "pages", "page_size", "max_pages", "layers", "page_bytes")] + \
+               [(n, C.c_int32) for n in ("op", "ids_arg", "aux_arg", "table_arg", "lens_arg", "refs_arg", "pool_arg",
+                                         "pad0")]
+
+
 class Params(C.Union):
     _fields_ = [("ew", EwParams), ("row", RowParams), ("qk", QkParams), ("gemm", GemmParams),
                 ("attn", AttnParams), ("red", ReduceParams), ("sel", SelectParams), ("gat", GatherParams),
-                ("ggemm", GGemmParams), ("gsum", GsumParams), ("itab", ItabParams)]
+                ("ggemm", GGemmParams), ("gsum", GsumParams), ("itab", ItabParams), ("pattn", PackedAttnParams),
+                ("kv4", Kv4Params), ("pages", PagesParams)]
 
 
 class Desc(C.Structure):
@@ -275,6 +307,18 @@ def describe(d):
         out.update(rows=q.rows, cols=q.cols,
                    outputs=[(ITAB_MODE_NAME.get(o.mode, o.mode), o.arg, o.map, o.reg) for o in list(q.out)[:q.nout]],
                    program=[(IOP_NAME.get(i.op, i.op), i.dst, i.a, i.b, i.c, i.imm) for i in list(q.code)[:q.ncode]])
+    elif d.kind == ATTN_PACKED:
+        a = d.p.pattn
+        out.update(q_tokens=a.q_tokens, k_tokens=a.k_tokens, seqs=a.seqs, hq=a.hq, hkv=a.hkv, dim=a.dim, scale=a.scale)
+    elif d.kind in (KV4_STORE, KV4_LOAD, ATTN_KV4):
+        q = d.p.kv4
+        out.update(slots=q.slots, hkv=q.hkv, dim=q.dim, group=q.group, pages=q.pages, page_size=q.page_size,
+                   max_pages=q.max_pages, layers=q.layers, layer=q.layer)
+        out.update(dict(hq=q.hq, scale=q.scale) if d.kind == ATTN_KV4 else dict(tokens=q.tokens))
+    elif d.kind == PAGES:
+        q = d.p.pages
+        out.update(op=PAGES_OP_NAME.get(q.op, q.op), n=q.n, slots=q.slots, pages=q.pages, page_size=q.page_size,
+                   max_pages=q.max_pages, layers=q.layers, page_bytes=q.page_bytes)
     elif d.kind == REDUCE_ALL:
         out.update(numel=d.p.red.numel, op="max" if d.p.red.op == RED_MAX else "sum")
         if d.p.red.pro.ncode:

@@ -66,23 +66,29 @@ def split(total, n):
 _workspaces = {}
 
 
-def workspace_for(blob, device):
-    """Scratch a launch of `blob` wants on `device` (split-K partials, reduction partials), as a device
-    tensor kept per device and grown on demand (or None)."""
+def workspace_for(blob, device, stream=None):
+    """Scratch a launch of `blob` wants on `device` (split-K partials, reduction partials), as a device tensor (or None).
+    It is kept per device and stream and grown on demand, so launches on two streams never share one; a launch that is
+    being captured gets one of its own from the capture's memory, which lives as long as the graph."""
     n = native.workspace_size(blob, device.index if device.index is not None else 0)
     if n <= 0:
         return None
     torch = _torch()
-    ws = _workspaces.get(device)
+    s = stream if stream is not None else torch.cuda.current_stream(device)
+    if torch.cuda.is_current_stream_capturing():
+        return torch.empty(int(n), dtype=torch.uint8, device=device)
+    key = (device, s.cuda_stream)
+    ws = _workspaces.get(key)
     if ws is None or ws.numel() < n:
-        ws = _workspaces[device] = torch.empty(int(n), dtype=torch.uint8, device=device)
+        ws = _workspaces[key] = torch.empty(int(n), dtype=torch.uint8, device=device)
+        ws.record_stream(s)
     return ws
 
 
 def launch_tensors(blob, tensors, lo=0, hi=None, stream=None, sync=True):
     """Run units [lo, hi) of descriptor `blob` over CUDA tensors (argument order), on `stream` (torch's
     current stream by default).  Tensors are used in place.  With sync=True, waits and checks the device
-    status word."""
+    status word; with sync=False the launch can be captured into a CUDA graph once its device has run one."""
     torch = _torch()
     desc = D.from_bytes(blob)
     if len(tensors) != desc.nargs:
@@ -100,9 +106,9 @@ def launch_tensors(blob, tensors, lo=0, hi=None, stream=None, sync=True):
             raise CudaError("every argument of one launch is on one device")
     hi = desc.units if hi is None else hi
     with torch.cuda.device(dev):
-        native.init(dev.index)
+        native.prepare(dev.index)
         s = stream if stream is not None else torch.cuda.current_stream(dev)
-        ws = workspace_for(blob, dev)
+        ws = workspace_for(blob, dev, s)
         native.launch(blob, [t.data_ptr() for t in tensors], lo, hi,
                       ws.data_ptr() if ws is not None else 0, ws.numel() if ws is not None else 0, s.cuda_stream)
         if sync:
@@ -134,6 +140,19 @@ def written_args(desc):
         return [p.ggemm.c_arg]
     if k == D.GATHER_SUM:
         return [p.gsum.out_arg]
+    if k == D.ATTN_PACKED:
+        return [p.pattn.o_arg]
+    if k == D.KV4_STORE:
+        return [p.kv4.pool_arg]
+    if k == D.KV4_LOAD:
+        return [p.kv4.a_arg, p.kv4.b_arg]
+    if k == D.ATTN_KV4:
+        return [p.kv4.b_arg]
+    if k == D.PAGES:
+        books = [p.pages.table_arg, p.pages.lens_arg, p.pages.refs_arg]
+        if p.pages.op == D.PAGES_OP["compact"]:
+            return [p.pages.table_arg, p.pages.refs_arg, p.pages.pool_arg]
+        return books + ([p.pages.pool_arg] if p.pages.pool_arg >= 0 else [])
     if k == D.INT_TABLE:
         return sorted({o.arg for o in list(p.itab.out)[:p.itab.nout]})
     raise CudaError(f"descriptor kind {k} ({D.KIND_NAME.get(k, 'unknown')}) has no known outputs")
@@ -172,7 +191,7 @@ class HostPipeline:
         outs = written_args(desc)
         dev = [torch.empty(t.numel(), dtype=t.dtype, device=self.device) for t in host]
         ptrs = [t.data_ptr() for t in dev]
-        ws = workspace_for(blob, self.device)
+        ws = workspace_for(blob, self.device, self.s_run)
         wsp, wsn = (ws.data_ptr(), ws.numel()) if ws is not None else (0, 0)
         self._live.append((dev, ws))
         # One native call enqueues the copies in, the kernels and the copies back (a row launch in pipelined unit

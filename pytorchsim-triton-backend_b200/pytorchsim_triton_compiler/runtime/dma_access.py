@@ -235,6 +235,55 @@ def _itab(d, lo, hi, names):
     return out
 
 
+def _ints(arg, n):
+    return (arg, "read", _box(0, [(n, 1)]))
+
+
+def _rows_through(tables, rows, elems, names):
+    return {"indirect": {"through": [names[t] for t in tables], "rows": int(rows), "row_elems": int(elems)}}
+
+
+def _packed(d, names):
+    a = d.p.pattn
+    cu = sorted({a.cuq_arg, a.cuk_arg})
+    q, k = (_rows_through([t], n * h, a.dim, names) for t, n, h in ((a.cuq_arg, a.q_tokens, a.hq), (a.cuk_arg, a.k_tokens, a.hkv)))
+    return [_ints(t, a.seqs + 1) for t in cu] + [(a.q_arg, "read", q), (a.k_arg, "read", k), (a.v_arg, "read", k),
+                                                 (a.o_arg, "write", q)]
+
+
+def _kv4(d, names):
+    """Token rows and records are found through the tables: at most `tokens` rows, or every row of the page table."""
+    q = d.p.kv4
+    out = [_ints(q.lens_arg, q.slots), _ints(q.table_arg, q.slots * q.max_pages)]
+    token = q.hkv * (q.dim + 8 * (q.dim // q.group))
+    if d.kind == D.ATTN_KV4:
+        row = _box(0, [(q.slots, q.a_row), (q.hq, q.a_head), (q.dim, 1)])
+        pool = _rows_through([q.lens_arg, q.table_arg], q.slots * q.max_pages, token * q.page_size, names)
+        return out + [(q.a_arg, "read", row), (q.pool_arg, "read", pool),
+                      (q.b_arg, "write", _box(0, [(q.slots, q.b_row), (q.hq, q.b_head), (q.dim, 1)]))]
+    out.append(_ints(q.cu_arg, q.slots + 1))
+    dense = _rows_through([q.cu_arg], q.tokens * q.hkv, q.dim, names)
+    pool = _rows_through([q.cu_arg, q.lens_arg, q.table_arg], q.tokens, token, names)
+    store = d.kind == D.KV4_STORE
+    return out + [(q.pool_arg, "write" if store else "read", pool), (q.a_arg, "read" if store else "write", dense),
+                  (q.b_arg, "read" if store else "write", dense)]
+
+
+def _page_books(d, names):
+    """The tables whole; the pages an operation copies are found through them."""
+    q = d.p.pages
+    tables = [(q.table_arg, q.slots * q.max_pages), (q.lens_arg, q.slots), (q.refs_arg, q.pages)]
+    out = [_ints(a, q.n) for a in (q.ids_arg, q.aux_arg) if a >= 0]
+    for arg, n in tables:
+        out.append(_ints(arg, n))
+        if arg != q.lens_arg or q.op != D.PAGES_OP["compact"]:
+            out.append((arg, "write", _box(0, [(n, 1)])))
+    if q.pool_arg >= 0:
+        moved = _rows_through([a for a, _ in tables], q.pages * q.layers, q.page_bytes, names)
+        out += [(q.pool_arg, "read", moved), (q.pool_arg, "write", moved)]
+    return out
+
+
 def streams(desc, lo, hi, names, dtypes=None, host=None):
     """The access streams of units [lo, hi) of `desc`, arguments named by `names` (argument order)."""
     d = desc
@@ -261,6 +310,12 @@ def streams(desc, lo, hi, names, dtypes=None, host=None):
         raw = _gsum(d, lo, hi, names)
     elif k == D.INT_TABLE:
         raw = _itab(d, lo, hi, names)
+    elif k == D.ATTN_PACKED:
+        raw = _packed(d, names)
+    elif k in (D.KV4_STORE, D.KV4_LOAD, D.ATTN_KV4):
+        raw = _kv4(d, names)
+    elif k == D.PAGES:
+        raw = _page_books(d, names)
     else:
         raise ValueError(f"no DMA-access plan for descriptor kind {k}")
     return [{"arg": names[a], "dir": direction, "dtype": (dtypes or {}).get(names[a]), "access": acc,

@@ -34,6 +34,16 @@ class Graph:
             t.copy_(init.reshape(-1).to(dt))
         return t
 
+    def bind(self, name, tensor):
+        """The caller's own device tensor as buffer `name` (contiguous, on this graph's device); returns the name."""
+        if not tensor.is_cuda or not tensor.is_contiguous() or tensor.device.index != (self.device.index or 0):
+            raise ValueError(f"buffer {name}: a contiguous tensor on {self.device} is required")
+        held = self.buffers.get(name)
+        if held is not None and held.data_ptr() != tensor.data_ptr():
+            raise ValueError(f"buffer {name} exists already")
+        self.buffers[name] = tensor
+        return name
+
     def add(self, name, blob, bufs, owners=None):
         """Append a launch of descriptor `blob` whose tensor arguments are the buffers `bufs`, in the
         descriptor's argument order; every buffer must exist with the descriptor's element count.  `owners`
@@ -63,8 +73,9 @@ class Graph:
         if self.cuda_graph is not None and stream is None:
             self.cuda_graph.replay()
         else:
-            for step in self.steps:
-                self._launch(step, s.cuda_stream)
+            with torch.cuda.device(self.device):
+                for step in self.steps:
+                    self._launch(step, s.cuda_stream)
         if sync:
             native.sync(s.cuda_stream)
 

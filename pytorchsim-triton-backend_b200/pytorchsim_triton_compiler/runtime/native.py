@@ -108,6 +108,13 @@ def init(device):
     _inited.add(int(device))
 
 
+def prepare(device):
+    """init(device) before this process's first launch there; nothing after that (init synchronises with the device, which
+    no later launch needs and a stream capture forbids)."""
+    if int(device) not in _inited:
+        init(device)
+
+
 def check(blob):
     """Validate a descriptor blob on the host (no GPU needed)."""
     buf = C.create_string_buffer(bytes(blob), len(blob))

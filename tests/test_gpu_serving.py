@@ -1,0 +1,757 @@
+"""The serving operators on the B200 against their definitions in 64 bits (oracle/serving.py and dense float64 products):
+packed prompt attention, the 4-bit paged cache, the page bookkeeping, and a serving loop of all of them.
+
+Tolerances, from the roundings that the kernels make (eps: the 16-bit type's; half a step is eps / 2):
+  - attention: each weight p_j is rounded to the type before it multiplies v_j, an error of at most eps / 2 of it, so a result
+    moves by at most eps / 2 times A = sum_j softmax_j |v_j|; the result itself is rounded, eps / 2 |o|.  The fp32 work (products
+    of 128 terms, the exponential, the sums) adds at most 2^-13 A: scores here are at most 2^4 with an error below
+    2^-20 of the sum of their absolute products (2^5 at most), 2^-15 twice, and the sums 2^-17.  fp16 adds half its
+    smallest step, 2^-25, where results are that small;
+  - over the cache: the rounded weight is p_j a_j (a: the V scale) and multiplies |code - 8| <= 8: eps / 2 * 8 sum_j softmax_j a_j in
+    the place of eps / 2 A;
+  - store: the record's bytes are those of the definition; load: one fp32 fma rounded to the type, eps / 2 of the value plus
+    2^-24 of scale * 15 + |minimum| for the fma;
+  - page bookkeeping: equal."""
+import math
+
+import pytest
+import torch
+
+from oracle import serving as S
+from pytorchsim_triton_compiler.codegen import build as B
+from pytorchsim_triton_compiler.codegen import descriptors as D
+from pytorchsim_triton_compiler.runtime import cuda as RC
+from pytorchsim_triton_compiler.runtime import native
+from pytorchsim_triton_compiler.runtime.graph import Graph
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bfloat16": torch.bfloat16, "float16": torch.float16}
+SMALLEST = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25}
+
+
+def gen(seed):
+    return torch.Generator().manual_seed(seed)
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32).cuda()
+
+
+def starts(lens, first=0):
+    out = [first]
+    for n in lens:
+        out.append(out[-1] + n)
+    return out
+
+
+def launch(desc, tensors, **kw):
+    return RC.launch_tensors(D.to_bytes(desc), tensors, **kw)
+
+
+def failed(desc, tensors):
+    with pytest.raises(native.ExecutorError) as e:
+        launch(desc, tensors)
+    return e.value.code
+
+
+# --------------------------------------------------------------------------------------------------------------------
+# Packed prompt attention
+# --------------------------------------------------------------------------------------------------------------------
+def dense(q, k, v, ql, kl, q0, k0, scale):
+    """(o, A) in float64 on the GPU: per sequence, per head."""
+    out, mag = torch.zeros(q.shape, dtype=torch.float64, device=q.device), torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    per = q.shape[1] // k.shape[1]
+    for s in range(len(ql)):
+        for h in range(q.shape[1]):
+            qq, kk, vv = (x[a:a + n, i].double() for x, a, n, i in ((q, q0[s], ql[s], h), (k, k0[s], kl[s], h // per), (v, k0[s], kl[s], h // per)))
+            place = torch.arange(ql[s], device=q.device)[:, None] + kl[s] - ql[s]
+            z = (qq @ kk.T * scale).masked_fill(torch.arange(kl[s], device=q.device)[None] > place, -math.inf)
+            p = torch.softmax(z, 1).nan_to_num(0.0) if kl[s] else z
+            out[q0[s]:q0[s] + ql[s], h], mag[q0[s]:q0[s] + ql[s], h] = p @ vv, p @ vv.abs()
+    return out, mag
+
+
+def near(got, want, mag, dtype, what=""):
+    half = torch.finfo(dtype).eps / 2
+    bound = half * (mag + want.abs()) + 2.0 ** -13 * mag + SMALLEST[dtype] + 1e-300
+    off = ((got.double() - want).abs() / bound)
+    assert bool((off <= 1).all()), f"{what}: {float(off.max()):.2f} of the bound at {divmod(int(off.argmax()), got.shape[-1])}"
+
+
+def packed_case(ql, kl, hq, hkv, dim, dtype, seed, gap=0, tail=0):
+    """Random rows; `gap` rows before the first sequence and `tail` after the last are in none."""
+    dt, g = DT[dtype], gen(seed)
+    q0, k0 = starts(ql, gap), starts(kl, gap)
+    q, k, v = (torch.randn(n, h, dim, generator=g).to(dt).cuda() for n, h in
+               ((q0[-1] + tail, hq), (k0[-1] + tail, hkv), (k0[-1] + tail, hkv)))
+    return q, k, v, q0, k0
+
+
+LENS = [[1], [2, 1, 3], [128], [129], [127, 1, 256], [257, 0, 255, 0, 0, 64], [0, 0, 300], [640, 33, 1, 511]]
+
+
+@pytest.mark.parametrize("dim,dtype,hq,hkv", [(128, "bfloat16", 4, 2), (64, "float16", 3, 1), (128, "float16", 2, 2), (64, "bfloat16", 8, 1)])
+@pytest.mark.parametrize("lens", LENS, ids=str)
+def test_packed_attention(lens, dim, dtype, hq, hkv):
+    q, k, v, q0, k0 = packed_case(lens, lens, hq, hkv, dim, dtype, sum(lens) + dim)
+    o = torch.full_like(q, 7.0)
+    launch(B.attention_packed(q0[-1], len(lens), hq, hkv, dim, dtype=dtype), [q, k, v, ints(q0), o])
+    near(o, *dense(q, k, v, lens, lens, q0, k0, 1 / math.sqrt(dim)), DT[dtype])
+
+
+@pytest.mark.parametrize("dim,dtype", [(128, "bfloat16"), (64, "float16")])
+@pytest.mark.parametrize("ql,kl", [([1], [1000]), ([5, 200], [5, 333]), ([300], [100]), ([129, 2, 7], [0, 1, 700]), ([256, 256], [511, 383]),
+                                   ([400], [1]), ([257], [256])], ids=str)
+def test_packed_attention_with_cached_prefixes(ql, kl, dim, dtype):
+    """More keys than queries (a chunk behind a prefix), fewer (rows that see nothing give zeros), none."""
+    q, k, v, q0, k0 = packed_case(ql, kl, 4, 2, dim, dtype, sum(kl))
+    o = torch.full_like(q, 7.0)
+    launch(B.attention_packed(q0[-1], len(ql), 4, 2, dim, dtype=dtype, k_tokens=k0[-1]), [q, k, v, ints(q0), ints(k0), o])
+    want, mag = dense(q, k, v, ql, kl, q0, k0, 1 / math.sqrt(dim))
+    near(o, want, mag, DT[dtype])
+    for s in range(len(ql)):
+        hidden = max(0, ql[s] - kl[s])
+        assert not o[q0[s]:q0[s] + hidden].any()
+
+
+def test_packed_attention_leaves_rows_outside_every_sequence():
+    lens = [100, 260]
+    q, k, v, q0, k0 = packed_case(lens, lens, 4, 4, 128, "bfloat16", 5, gap=37, tail=90)
+    for x in (q, k, v):                                   # what lies there may be anything
+        x[:37], x[397:] = float("nan"), float("inf")
+    o = torch.full_like(q, 7.0)
+    launch(B.attention_packed(q.shape[0], 2, 4, 4), [q, k, v, ints(q0), o])
+    want, mag = dense(q, k, v, lens, lens, q0, k0, 1 / math.sqrt(128))
+    near(o[37:397], want[37:397], mag[37:397], torch.bfloat16)
+    assert bool((o[:37] == 7).all()) and bool((o[397:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype,dim", [("bfloat16", 128), ("float16", 64)])
+def test_packed_attention_is_blind_to_keys_it_does_not_see(dtype, dim):
+    """Infinities and NaN in later keys and in other sequences do not reach a row; in keys it sees they do."""
+    lens = [70, 300, 200]
+    q, k, v, q0, k0 = packed_case(lens, lens, 2, 1, dim, dtype, 11)
+    clean = [x.clone() for x in (q, k, v)]
+    at = q0[1] + 150
+    v[at, 0, 3], v[at + 1, 0, 5], v[at + 2, 0, 5], v[at + 3, 0, dim - 1] = float("nan"), float("inf"), -float("inf"), -float("inf")
+    k[at + 20, 0, 1] = float("nan")
+    q[q0[2] + 5, 0] = float("inf")
+    o = torch.zeros_like(q)
+    launch(B.attention_packed(q0[-1], 3, 2, 1, dim, dtype=dtype), [q, k, v, ints(q0), o])
+    want, mag = dense(*clean, lens, lens, q0, k0, 1 / math.sqrt(dim))
+    fine = torch.ones(q0[-1], 2, dtype=torch.bool, device="cuda")
+    fine[at:q0[2]] = False
+    fine[q0[2] + 5, 0] = False
+    near(o[fine], want[fine], mag[fine], DT[dtype])
+    rows = o[at:at + 20].float()                          # from the first bad value to the bad key
+    assert rows[:, :, 3].isnan().all()
+    assert bool((rows[1, :, 5] == math.inf).all()) and rows[2:, :, 5].isnan().all() and bool((rows[3:, :, dim - 1] == -math.inf).all())
+    others = [d for d in range(dim) if d not in (3, 5, dim - 1)]
+    near(o[at:at + 20][:, :, others], want[at:at + 20][:, :, others], mag[at:at + 20][:, :, others], DT[dtype])
+    assert rows[0, :, 5].isfinite().all() and o[at + 20:q0[2]].isnan().all() and o[q0[2] + 5, 0].isnan().all()
+
+
+@pytest.mark.parametrize("scale", [1e-3, 1.0, 40.0])
+def test_packed_attention_of_flat_and_peaked_rows(scale):
+    """Equal weights, and rows that one key takes whole (its reference moves often).  At scale 40 a score is up to 40 * 60 with an
+    error of 2^-20 of 40 * 100 absolute products, 2^-8: the rows' weights are then known to 2^-7 only, which the bound gets."""
+    q, k, v, q0, k0 = packed_case([700], [700], 2, 1, 128, "bfloat16", 3)
+    o = torch.zeros_like(q)
+    launch(B.attention_packed(700, 1, 2, 1, scale=scale), [q, k, v, ints(q0), o])
+    want, mag = dense(q, k, v, [700], [700], q0, k0, scale)
+    near(o, want, mag * (1 if scale <= 1 else 3), torch.bfloat16, f"scale {scale}")
+
+
+def test_packed_attention_of_scores_far_below_zero():
+    """Rows whose every score is -2^27 have equal weights, whatever a mask's lowest value may be elsewhere."""
+    q, k, v, q0, k0 = packed_case([200], [200], 1, 1, 64, "bfloat16", 4)
+    q.fill_(-2.0 ** 12)
+    k.fill_(2.0 ** 12)
+    o = torch.zeros_like(q)
+    launch(B.attention_packed(200, 1, 1, 1, 64), [q, k, v, ints(q0), o])
+    near(o, *dense(q, k, v, [200], [200], q0, k0, 1 / 8), torch.bfloat16)
+
+
+def test_packed_attention_of_one_long_prompt():
+    n = 20001
+    q, k, v, q0, _ = packed_case([n], [n], 1, 1, 128, "bfloat16", 6)
+    o = torch.zeros_like(q)
+    launch(B.attention_packed(n, 1, 1, 1), [q, k, v, ints(q0), o])
+    for row in (0, 127, 128, 9999, n - 2, n - 1):
+        p = torch.softmax(q[row, 0].double() @ k[:row + 1, 0].double().T / math.sqrt(128), 0)
+        near(o[row, 0], p @ v[:row + 1, 0].double(), p @ v[:row + 1, 0].double().abs(), torch.bfloat16, f"row {row}")
+
+
+@pytest.mark.parametrize("layout", ["fused", "head_major"])
+def test_packed_attention_layouts_agree_bit_for_bit(layout):
+    lens, hq, hkv = [130, 5, 259], 8, 2
+    q, k, v, q0, _ = packed_case(lens, lens, hq, hkv, 128, "bfloat16", 8)
+    n, a = q0[-1], torch.zeros_like(q)
+    launch(B.attention_packed(n, 3, hq, hkv), [q, k, v, ints(q0), a])
+    b = torch.zeros_like(q)
+    if layout == "fused":
+        launch(B.attention_packed(n, 3, hq, hkv, fused=True), [torch.cat([q, k, v], 1).contiguous(), ints(q0), b])
+    else:
+        heads = [x.transpose(0, 1).contiguous() for x in (q, k, v, b)]
+        launch(B.attention_packed(n, 3, hq, hkv, head_major=True), [*heads[:3], ints(q0), heads[3]])
+        b = heads[3].transpose(0, 1)
+    assert torch.equal(a, b)
+
+
+def test_packed_attention_of_many_sequences():
+    lens = [(7 * i) % 5 for i in range(D.PACKED_SEQS)]
+    q, k, v, q0, k0 = packed_case(lens, lens, 1, 1, 64, "bfloat16", 9)
+    o = torch.zeros_like(q)
+    launch(B.attention_packed(q0[-1], len(lens), 1, 1, 64), [q, k, v, ints(q0), o])
+    some = [i for i in range(len(lens)) if i % 97 == 0 or i > len(lens) - 6]
+    want, mag = dense(q, k, v, [lens[i] for i in some], [lens[i] for i in some], [q0[i] for i in some], [k0[i] for i in some], 1 / 8)
+    rows = [r for i in some for r in range(q0[i], q0[i + 1])]
+    near(o[rows], want[rows], mag[rows], torch.bfloat16)
+
+
+@pytest.mark.parametrize("table", [[0, 50, 40, 100], [0, 50, 60, 101], [-1, 50, 60, 100]])
+def test_packed_attention_reports_a_bad_table(table):
+    """The sequence with the bad entries is skipped, the others are computed."""
+    q, k, v, _, _ = packed_case([100], [100], 2, 1, 64, "bfloat16", 10)
+    o = torch.full_like(q, 7.0)
+    assert failed(B.attention_packed(100, 3, 2, 1, 64), [q, k, v, ints(table), o]) == D.E_OOB
+    if table[0] == 0:
+        want, mag = dense(q, k, v, [50], [50], [0], [0], 1 / 8)
+        near(o[:40], want[:40], mag[:40], torch.bfloat16)
+
+
+def test_packed_attention_of_nothing():
+    q = torch.zeros(0, 2, 64, dtype=torch.bfloat16, device="cuda")
+    launch(B.attention_packed(0, 2, 2, 2, 64), [q, q, q, ints([0, 0, 0]), q])
+    q, k, v, q0, _ = packed_case([3], [3], 2, 1, 64, "bfloat16", 12)
+    o = torch.full_like(q, 7.0)
+    launch(B.attention_packed(3, 0, 2, 1, 64), [q, k, v, ints([0]), o])
+    assert bool((o == 7).all())
+
+
+# --------------------------------------------------------------------------------------------------------------------
+# The 4-bit cache
+# --------------------------------------------------------------------------------------------------------------------
+def cache_case(lens, dim, page, group, hkv, dtype, seed, layers=1, spare=2):
+    """A shape, a table of shuffled pages and an empty pool of a recognisable byte."""
+    g = gen(seed)
+    held = [-(-n // page) for n in lens]
+    width, pages = max(1, max(held)), sum(held) + spare
+    order = torch.randperm(pages, generator=g).tolist()
+    table, at = [], 0
+    for n in held:
+        table.append(order[at:at + n] + [-1] * (width - n))
+        at += n
+    c = B.kv4_cache(slots=len(lens), max_pages=width, pages=pages, hkv=hkv, dim=dim, page_size=page, group=group, layers=layers, dtype=dtype)
+    return c, table, torch.full((c.pool_bytes,), 0xA5, dtype=torch.uint8, device="cuda")
+
+
+def rows_of(n, c, seed, spread=1.0):
+    g = gen(seed)
+    return [(torch.randn(n, c.hkv, c.dim, generator=g) * spread + x).to(DT[c.dtype]).cuda() for x in (0.5, -0.25)]
+
+
+SHAPES = [(128, 16, 64, 2, "bfloat16"), (128, 16, 32, 1, "float16"), (128, 32, 128, 3, "bfloat16"), (128, 64, 64, 1, "float16"),
+          (128, 128, 32, 1, "bfloat16"), (64, 16, 64, 3, "float16"), (64, 32, 32, 1, "bfloat16"), (64, 128, 64, 2, "bfloat16")]
+
+
+@pytest.mark.parametrize("dim,page,group,hkv,dtype", SHAPES)
+def test_store_writes_the_defined_bytes_and_load_reads_them(dim, page, group, hkv, dtype):
+    new, old = [1, 0, page + 3, 7], [page - 1, 4, 5, 0]              # across a page's end, none, several pages, a fresh slot
+    lens = [a + b for a, b in zip(new, old)]
+    c, table, pool = cache_case(lens, dim, page, group, hkv, dtype, page + dim, layers=2)
+    k, v = rows_of(sum(new), c, 3)
+    k[0, 0, :group] = 1.5                                            # a constant group
+    v[1, 0, 0] = float("nan")
+    k[2, 0, dim - 1] = -float("inf")
+    want = S.Cache(c, pool.cpu(), table, lens)
+    row = 0
+    for s in range(4):
+        for i in range(new[s]):
+            for h in range(hkv):
+                want.write(s, old[s] + i, h, k[row, h].cpu(), v[row, h].cpu(), layer=1)
+            row += 1
+    books = [ints(lens), ints(table), pool]
+    launch(B.kv4_store(c, sum(new), layer=1), [k, v, ints(starts(new))] + books)
+    got = pool.cpu().view(want.pool.shape)
+    bad = (got != want.pool).nonzero()
+    # A NaN's bits are free: compare those parameters by what they stand for, everything else by its bytes.
+    back = S.Cache(c, pool.cpu(), table, lens)
+    kb, vb = torch.zeros_like(k), torch.zeros_like(v)
+    launch(B.kv4_load(c, sum(new), layer=1), [ints(starts(new))] + books + [kb, vb])
+    row = 0
+    for s in range(4):
+        for i in range(new[s]):
+            for h in range(hkv):
+                for x, y, z in zip(back.read(s, old[s] + i, h, 1), want.read(s, old[s] + i, h, 1), (kb, vb)):
+                    assert torch.equal(x.isnan(), y.isnan()) and torch.equal(x.nan_to_num(0), y.nan_to_num(0))
+                    z = z[row, h].cpu().double()
+                    assert torch.equal(z.isnan(), y.isnan())
+                    y = y.nan_to_num(0)
+                    lim = torch.finfo(DT[dtype]).eps / 2 * y.abs() + 2.0 ** -24 * 64 + SMALLEST[DT[dtype]]
+                    assert bool(((z.nan_to_num(0) - y).abs() <= lim).all())
+            row += 1
+    assert len(bad) <= 8, f"{len(bad)} bytes differ from the definition"     # at most the two NaN pairs
+    assert bool((got[0] == 0xA5).all())                                       # the other layer
+
+
+def test_store_and_load_skip_and_report_what_has_no_place():
+    lens = [20, 20, 40, 5]
+    c, table, pool = cache_case(lens, 128, 16, 64, 1, "bfloat16", 1)
+    k, v = rows_of(12, c, 5)
+    table[1][1] = c.pages                                       # a page outside the pool
+    table[2][2] = -1
+    lens[3] = -2                                                # a length that cannot be
+    before = pool.clone()
+    cu, books = ints([0, 3, 6, 9, 12]), [ints(lens), ints(table), pool]
+    assert failed(B.kv4_store(c, 12), [k, v, cu] + books) == D.E_OOB
+    changed = (pool != before).view(c.pages, -1).any(1).nonzero().flatten().tolist()
+    assert changed == [table[0][1]]
+    kb, vb = torch.full_like(k, 3.0), torch.full_like(v, 3.0)
+    assert failed(B.kv4_load(c, 12), [cu] + books + [kb, vb]) == D.E_OOB
+    assert not kb[3:12].any() and not vb[3:12].any() and kb[:3].any()
+    # rows outside every slot are left alone
+    kb.fill_(3.0)
+    launch(B.kv4_load(c, 12), [ints([2, 4, 4, 4, 4])] + books + [kb, vb])
+    assert bool((kb[:2] == 3).all()) and bool((kb[4:] == 3).all()) and bool((kb[2:4] != 3).any())
+
+
+def test_store_takes_a_fused_projection_and_head_major_keys():
+    new = [5, 18]
+    c, table, pool = cache_case(new, 128, 16, 64, 2, "bfloat16", 2)
+    k, v = rows_of(23, c, 6)
+    other = [pool.clone(), pool.clone()]
+    cu, books = ints(starts(new)), [ints(new), ints(table)]
+    launch(B.kv4_store(c, 23), [k, v, cu] + books + [pool])
+    q = torch.randn(23, 6, 128, device="cuda").to(torch.bfloat16)
+    launch(B.kv4_store(c, 23, fused_hq=6), [torch.cat([q, k, v], 1).contiguous(), cu] + books + [other[0]])
+    launch(B.kv4_store(c, 23, head_major=True), [k.transpose(0, 1).contiguous(), v, cu] + books + [other[1]])
+    assert torch.equal(pool, other[0]) and torch.equal(pool, other[1])
+
+
+def cache_attention(q, k, v, lens, group, scale):
+    """(o, bound on the weights' rounding / (eps / 2)) in float64, from the dense rows of each slot."""
+    per = q.shape[1] // k.shape[1]
+    out, mag = torch.zeros(q.shape, dtype=torch.float64, device=q.device), torch.zeros(q.shape, dtype=torch.float64, device=q.device)
+    at = starts(lens)
+    for s, n in enumerate(lens):
+        for h in range(k.shape[1] if n else 0):
+            kk, vv = (S.dequantised(x[at[s]:at[s + 1], h], group) for x in (k, v))
+            a = S.quantise(v[at[s]:at[s + 1], h], group)[1].double().repeat_interleave(group, -1)
+            rows = slice(h * per, (h + 1) * per)
+            p = torch.softmax(q[s, rows].double() @ kk.T * scale, 1)
+            out[s, rows], mag[s, rows] = p @ vv, 8 * (p @ a) + 0 * (p @ vv)
+    return out, mag
+
+
+ATTN = [(128, 16, 64, 2, 4, "bfloat16"), (128, 16, 32, 1, 8, "float16"), (128, 32, 128, 2, 1, "bfloat16"), (128, 64, 64, 1, 9, "float16"),
+        (128, 128, 32, 1, 16, "bfloat16"), (64, 16, 64, 3, 3, "float16"), (64, 32, 32, 1, 17, "bfloat16"), (64, 128, 64, 2, 40, "bfloat16"),
+        (128, 32, 64, 1, 12, "bfloat16")]
+CONTEXTS = [[1], [0], [31, 0, 32, 33, 1, 16, 17, 64], [1000, 3, 129], [15] * 70]
+
+
+@pytest.mark.parametrize("dim,page,group,hkv,per,dtype", ATTN)
+@pytest.mark.parametrize("lens", CONTEXTS, ids=lambda x: str(x[:9]))
+def test_cache_attention(dim, page, group, hkv, per, dtype, lens):
+    c, table, pool = cache_case(lens, dim, page, group, hkv, dtype, sum(lens) + page)
+    k, v = rows_of(sum(lens), c, 8)
+    q = torch.randn(len(lens), hkv * per, dim, generator=gen(9)).to(DT[dtype]).cuda()
+    books = [ints(lens), ints(table), pool]
+    launch(B.kv4_store(c, sum(lens)), [k, v, ints(starts(lens))] + books)
+    o = torch.full_like(q, 7.0)
+    launch(B.attention_kv4(c, hkv * per), [q] + books + [o])
+    want, mag = cache_attention(q, k, v, lens, group, 1 / math.sqrt(dim))
+    near(o, want, mag, DT[dtype])
+    for s, n in enumerate(lens):
+        assert n or not o[s].any()
+
+
+@pytest.mark.parametrize("dtype,page", [("bfloat16", 16), ("float16", 64)])
+def test_cache_attention_of_a_long_context(dtype, page):
+    """100000 keys, whose weights average out: the result is 2^-8 of the values, and its error has to follow."""
+    lens = [100001, 40]
+    c, table, pool = cache_case(lens, 128, page, 64, 1, dtype, 4)
+    k, v = rows_of(sum(lens), c, 10)
+    v += 0.25                                                  # about zero
+    q = torch.randn(2, 4, 128, generator=gen(11)).to(DT[dtype]).cuda()
+    books = [ints(lens), ints(table), pool]
+    launch(B.kv4_store(c, sum(lens)), [k, v, ints(starts(lens))] + books)
+    o = torch.zeros_like(q)
+    launch(B.attention_kv4(c, 4), [q] + books + [o])
+    want, mag = cache_attention(q, k, v, lens, 64, 1 / math.sqrt(128))
+    near(o, want, mag, DT[dtype])
+    rel = (o.double() - want)[0].norm() / want[0].norm()
+    # Independent roundings: each weight's is uniform within half a step, 1 / sqrt(3) of it on average, and meets a code whose distance
+    # from 8 averages like the values themselves; the result's own rounding is the same size.  Four times their sum.
+    assert rel < 4 * torch.finfo(DT[dtype]).eps / math.sqrt(3), rel
+
+
+def test_cache_attention_ignores_what_lies_behind_a_slot():
+    """The rest of the last page, other pages and a forked neighbour hold NaN parameters."""
+    lens = [33, 5]
+    for page in (16, 32, 64):
+        c, table, pool = cache_case(lens, 128, page, 64, 2, "bfloat16", page)
+        pool.fill_(0xFF)                                       # every parameter a NaN
+        k, v = rows_of(sum(lens), c, 12)
+        q = torch.randn(2, 8, 128, generator=gen(13)).to(torch.bfloat16).cuda()
+        books = [ints(lens), ints(table), pool]
+        launch(B.kv4_store(c, sum(lens)), [k, v, ints(starts(lens))] + books)
+        o = torch.zeros_like(q)
+        launch(B.attention_kv4(c, 8), [q] + books + [o])
+        near(o, *cache_attention(q, k, v, lens, 64, 1 / math.sqrt(128)), torch.bfloat16)
+
+
+def test_cache_attention_passes_on_non_finite_keys_and_values_it_sees():
+    lens = [40, 40, 40]
+    c, table, pool = cache_case(lens, 64, 16, 32, 1, "bfloat16", 5)
+    k, v = rows_of(120, c, 14)
+    k[10, 0, 0] = float("nan")
+    v[50, 0, 40] = float("inf")
+    q = torch.randn(3, 2, 64, generator=gen(15)).to(torch.bfloat16).cuda()
+    books = [ints(lens), ints(table), pool]
+    launch(B.kv4_store(c, 120), [k, v, ints(starts(lens))] + books)
+    o = torch.zeros_like(q)
+    launch(B.attention_kv4(c, 2), [q] + books + [o])
+    want, mag = cache_attention(q, k, v, lens, 32, 1 / 8)
+    assert o[0].isnan().all() and o[1, :, 32:].isnan().all()
+    near(o[1, :, :32], want[1, :, :32], mag[1, :, :32], torch.bfloat16)
+    near(o[2], want[2], mag[2], torch.bfloat16)
+
+
+@pytest.mark.parametrize("page,dtype", [(16, "bfloat16"), (64, "float16")])
+def test_cache_attention_of_flat_and_peaked_rows(page, dtype):
+    lens = [700, 65]
+    c, table, pool = cache_case(lens, 128, page, 64, 1, dtype, 6)
+    k, v = rows_of(sum(lens), c, 16)
+    q = torch.randn(2, 8, 128, generator=gen(17)).to(DT[dtype]).cuda()
+    books = [ints(lens), ints(table), pool]
+    launch(B.kv4_store(c, sum(lens)), [k, v, ints(starts(lens))] + books)
+    for scale in (1e-4, 1.0):
+        o = torch.zeros_like(q)
+        launch(B.attention_kv4(c, 8, scale=scale), [q] + books + [o])
+        near(o, *cache_attention(q, k, v, lens, 64, scale), DT[dtype], f"scale {scale}")
+
+
+def test_cache_attention_of_wide_values_in_fp16():
+    """V scales of thousands times weights: no operand leaves fp16."""
+    lens = [90]
+    c, table, pool = cache_case(lens, 128, 16, 64, 1, "float16", 7)
+    k, v = rows_of(90, c, 18)
+    v[:, :, ::2], v[:, :, 1::2] = -60000.0, 60000.0
+    v[::3] *= 0.5
+    q = (torch.randn(1, 8, 128, generator=gen(19)) * 4).to(torch.float16).cuda()
+    books = [ints(lens), ints(table), pool]
+    launch(B.kv4_store(c, 90), [k, v, ints([0, 90])] + books)
+    o = torch.zeros_like(q)
+    launch(B.attention_kv4(c, 8), [q] + books + [o])
+    near(o, *cache_attention(q, k, v, lens, 64, 1 / math.sqrt(128)), torch.float16)
+
+
+def test_cache_attention_reports_bad_pages_and_lengths():
+    """A page outside the pool is not attended to, a length outside the row gives zeros; other slots are computed."""
+    lens = [40, 40, 40]
+    c, table, pool = cache_case(lens, 128, 16, 64, 1, "bfloat16", 8)
+    k, v = rows_of(120, c, 20)
+    q = torch.randn(3, 4, 128, generator=gen(21)).to(torch.bfloat16).cuda()
+    launch(B.kv4_store(c, 120), [k, v, ints(starts(lens)), ints(lens), ints(table), pool])
+    table[0][1] = -5                                            # keys 16 .. 31 of slot 0 are lost
+    o = torch.zeros_like(q)
+    assert failed(B.attention_kv4(c, 4), [q, ints([40, 49, 40]), ints(table), pool, o]) == D.E_OOB
+    keep = [t for t in range(120) if not 16 <= t < 32]
+    want, mag = cache_attention(q, k[keep], v[keep], [24, 40, 40], 64, 1 / math.sqrt(128))
+    near(o[[0, 2]], want[[0, 2]], mag[[0, 2]], torch.bfloat16)
+    assert not o[1].any()
+
+
+def test_cache_attention_takes_a_fused_projection():
+    lens = [50, 20]
+    c, table, pool = cache_case(lens, 128, 16, 64, 2, "bfloat16", 9)
+    k, v = rows_of(70, c, 22)
+    q = torch.randn(2, 8, 128, generator=gen(23)).to(torch.bfloat16).cuda()
+    books = [ints(lens), ints(table), pool]
+    launch(B.kv4_store(c, 70), [k, v, ints(starts(lens))] + books)
+    a, b = torch.zeros_like(q), torch.zeros_like(q)
+    launch(B.attention_kv4(c, 8), [q] + books + [a])
+    launch(B.attention_kv4(c, 8, fused=True), [torch.cat([q, k[:2], v[:2]], 1).contiguous()] + books + [b])
+    assert torch.equal(a, b)
+
+
+# --------------------------------------------------------------------------------------------------------------------
+# Page bookkeeping
+# --------------------------------------------------------------------------------------------------------------------
+class Live:
+    """The device state beside the oracle's."""
+
+    def __init__(self, slots=6, width=5, pages=23, page=16, layers=2, hkv=1):
+        self.c = B.kv4_cache(slots=slots, max_pages=width, pages=pages, hkv=hkv, dim=64, page_size=page, group=64, layers=layers)
+        self.table, self.lens, self.refs = ints([[-1] * width] * slots), ints([0] * slots), ints([0] * pages)
+        self.pool = torch.randint(0, 256, (layers, pages, self.c.page_bytes), generator=gen(pages), dtype=torch.uint8).cuda()
+        self.want = S.Pages(self.table.tolist(), [0] * slots, [0] * pages, self.pool.cpu(), page)
+
+    def books(self):
+        return [self.table, self.lens, self.refs]
+
+    def same(self):
+        assert self.table.tolist() == self.want.table and self.lens.tolist() == self.want.lens
+        assert self.refs.tolist() == self.want.refs and torch.equal(self.pool.cpu(), self.want.pool)
+
+    def grow(self, ids, add):
+        launch(B.pages_grow(self.c, len(ids)), [ints(ids), ints(add)] + self.books())
+        self.want.grow(ids, add)
+        self.same()
+
+    def fork(self, src, dst, deep=False):
+        launch(B.pages_fork(self.c, len(src), deep), [ints(src), ints(dst)] + self.books() + [self.pool])
+        self.want.fork(src, dst, deep)
+        self.same()
+
+    def free(self, ids):
+        launch(B.pages_free(self.c, len(ids)), [ints(ids)] + self.books())
+        self.want.free(ids)
+        self.same()
+
+    def compact(self):
+        launch(B.pages_compact(self.c), self.books() + [self.pool])
+        self.want.compact()
+        self.same()
+
+
+def test_pages_by_hand():
+    a = Live()
+    a.grow([2, 0], [17, 16])                  # two pages, one page
+    a.grow([0, 2, 1], [0, 15, 1])             # nothing, to the end of a page, a fresh slot
+    a.fork([2, 0], [3, 4])                    # full pages only: nothing is copied
+    a.grow([2, 0], [1, 3])                    # past the shared pages: pages of their own
+    a.fork([2], [5])
+    a.free([2, 1, 2])                         # one slot listed twice
+    a.compact()
+    a.compact()                               # nothing to move
+    a.fork([5, 0], [1, 2], deep=True)
+    a.free([5, 4, 3, 0])
+    a.compact()
+    a.free([1, 2])
+    assert not a.refs.any()
+
+
+@pytest.mark.parametrize("slots,width,pages,page", [(6, 5, 23, 16), (40, 3, 90, 32), (9, 700, 5001, 16), (300, 60, 16400, 16)])
+def test_pages_at_random(slots, width, pages, page):
+    """Any order of operations that fits, against the slot-by-slot bookkeeping."""
+    import random
+    rng = random.Random(slots)
+    a = Live(slots, width, pages, page)
+    for _ in range(14):
+        room = sum(r <= 0 for r in a.want.refs)
+        empty = [s for s in range(slots) if not a.want.lens[s]]
+        full = [s for s in range(slots) if a.want.lens[s]]
+        what = rng.choice(["grow", "grow", "fork", "copy", "free", "compact"])
+        if what == "grow":
+            ids = rng.sample(range(slots), rng.randint(1, slots))
+            add = [rng.randint(0, max(0, min(width * page - a.want.lens[s], max(0, room // len(ids) - 1) * page))) for s in ids]
+            a.grow(ids, add)
+        elif what in ("fork", "copy") and full and empty:
+            dst = rng.sample(empty, rng.randint(1, len(empty)))
+            src = [rng.choice(full) for _ in dst]
+            while dst and sum(a.want.held(a.want.lens[s]) if what == "copy" else 1 for s in src) > room:
+                src, dst = src[:-1], dst[:-1]
+            if dst:
+                a.fork(src, dst, what == "copy")
+        elif what == "free" and full:
+            a.free([rng.choice(full) for _ in range(rng.randint(1, len(full)))])
+        else:
+            a.compact()
+
+
+def test_pages_refuse_and_leave_everything_as_it_was():
+    a = Live(slots=5, width=4, pages=7, page=16)
+    a.grow([0, 1], [40, 20])                  # 3 + 2 pages of 7
+    ops = [
+        (B.pages_grow(a.c, 2), [[0, 5], [1, 1]], False, D.E_OOB),            # a slot outside
+        (B.pages_grow(a.c, 2), [[0, -1], [1, 1]], False, D.E_OOB),
+        (B.pages_grow(a.c, 2), [[2, 2], [1, 1]], False, D.E_ARGS),           # listed twice
+        (B.pages_grow(a.c, 2), [[2, 3], [1, -1]], False, D.E_ARGS),
+        (B.pages_grow(a.c, 2), [[2, 0], [1, 25]], False, D.E_RESOURCE),      # past the row
+        (B.pages_grow(a.c, 2), [[2, 3], [17, 20]], False, D.E_RESOURCE),     # 4 pages of the 2 free ones
+        (B.pages_grow(a.c, 2), [[2, 0], [1, 2 ** 31 - 1]], False, D.E_RESOURCE),
+        (B.pages_fork(a.c, 2), [[0, 1], [2, 2]], True, D.E_ARGS),            # one target twice
+        (B.pages_fork(a.c, 2), [[0, 0], [2, 1]], True, D.E_ARGS),            # a target in use
+        (B.pages_fork(a.c, 2), [[0, 3], [3, 4]], True, D.E_ARGS),            # a target that is a source
+        (B.pages_fork(a.c, 2), [[0, 1], [2, 7]], True, D.E_OOB),
+        (B.pages_fork(a.c, 1, True), [[0], [2]], True, D.E_RESOURCE),        # 3 pages of 2
+        (B.pages_free(a.c, 1), [[9]], False, D.E_OOB),
+    ]
+    for desc, lists, pool, code in ops:
+        n = len(lists[0])
+        assert failed(desc, [ints(x) for x in lists] + a.books() + ([a.pool] if pool else [])) == code, (lists, n)
+        a.same()
+    a.fork([0, 1], [2, 3])                    # the two partial pages take the two free ones
+    assert failed(B.pages_fork(a.c, 1), [ints([0]), ints([4])] + a.books() + [a.pool]) == D.E_RESOURCE
+    a.same()
+
+
+# --------------------------------------------------------------------------------------------------------------------
+# Together, and as programs use them
+# --------------------------------------------------------------------------------------------------------------------
+def test_a_serving_loop():
+    """Prompts admitted, attended and stored, decoded in a batch, forked, decoded apart, freed and compacted: the cache holds what a
+    dense history says at every step, and compaction changes no result."""
+    hq, hkv, dim, page, group = 8, 2, 128, 16, 64
+    c = B.kv4_cache(slots=5, max_pages=8, pages=24, hkv=hkv, dim=dim, page_size=page, group=group, layers=2)
+    g = gen(31)
+    table, lens, refs = ints([[-1] * 8] * 5), ints([0] * 5), ints([0] * 24)
+    pool = torch.zeros(c.pool_bytes, dtype=torch.uint8, device="cuda")
+    books, layer, scale = [table, lens, refs], 1, 1 / math.sqrt(dim)
+    past = [[] for _ in range(5)]             # (k, v) rows of every slot, dense
+
+    def project(n):
+        return torch.randn(n, hq + 2 * hkv, dim, generator=g).to(torch.bfloat16).cuda()
+
+    def admit(new):
+        """new: {slot: prompt length}."""
+        ids = sorted(new)
+        launch(B.pages_grow(c, len(ids)), [ints(ids), ints([new[s] for s in ids])] + books)
+        counts = [new.get(s, 0) for s in range(5)]
+        qkv, cu = project(sum(counts)), starts(counts)
+        o = torch.zeros(sum(counts), hq, dim, dtype=torch.bfloat16, device="cuda")
+        launch(B.attention_packed(sum(counts), 5, hq, hkv, fused=True), [qkv, ints(cu), o])
+        launch(B.kv4_store(c, sum(counts), layer, fused_hq=hq), [qkv, ints(cu), lens, table, pool])
+        q, k, v = (x.contiguous() for x in qkv.split([hq, hkv, hkv], 1))
+        near(o, *dense(q, k, v, counts, counts, cu, cu, scale), torch.bfloat16)
+        for s in ids:
+            past[s] += [(k[t], v[t]) for t in range(cu[s], cu[s + 1])]
+
+    def attend(q):
+        o = torch.full((5, hq, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+        launch(B.attention_kv4(c, hq, layer), [q, lens, table, pool, o])
+        return o
+
+    def decode(ids):
+        """One token for each of the slots `ids`; every slot attends."""
+        launch(B.pages_grow(c, len(ids)), [ints(ids), ints([1] * len(ids))] + books)
+        counts = [int(s in ids) for s in range(5)]
+        qkv = project(len(ids))
+        launch(B.kv4_store(c, len(ids), layer, fused_hq=hq), [qkv, ints(starts(counts)), lens, table, pool])
+        for row, s in enumerate(sorted(ids)):
+            past[s].append((qkv[row, hq:hq + hkv], qkv[row, hq + hkv:]))
+        q = torch.randn(5, hq, dim, generator=g).to(torch.bfloat16).cuda()
+        o = attend(q)
+        n = [len(p) for p in past]
+        assert lens.tolist() == n
+        k, v = (torch.stack([kv[i] for p in past for kv in p]) for i in (0, 1))
+        near(o, *cache_attention(q, k, v, n, group, scale), torch.bfloat16)
+        return q, o
+
+    admit({0: 37, 2: 16, 4: 1})
+    for _ in range(3):
+        decode([0, 2, 4])
+    launch(B.pages_fork(c, 2), [ints([0, 0]), ints([1, 3])] + books + [pool])
+    past[1], past[3] = list(past[0]), list(past[0])
+    for _ in range(2):
+        decode([0, 1, 2, 3, 4])               # the forks part ways
+    launch(B.pages_free(c, 2), [ints([0, 2])] + books)
+    past[0], past[2] = [], []
+    q, before = decode([1, 4])
+    launch(B.pages_compact(c), books + [pool])
+    assert torch.equal(attend(q), before)
+    admit({0: 90})
+    decode([0, 1, 3, 4])
+    live = int((refs > 0).sum())
+    assert sorted(set(table.flatten().tolist()) - {-1}) == torch.nonzero(refs > 0).flatten().tolist() and live <= 24
+
+
+def decode_graph(seed, slots=3):
+    lens = [50, 7, 33][:slots]
+    c, table, pool = cache_case(lens, 128, 16, 64, 2, "bfloat16", seed)
+    k, v = rows_of(sum(lens), c, seed)
+    q = torch.randn(slots, 8, 128, generator=gen(seed + 1)).to(torch.bfloat16).cuda()
+    o = torch.zeros_like(q)
+    books = [ints(lens), ints(table), pool]
+    g = Graph("cuda:0")
+    for n, t in zip(("k", "v", "cu", "lens", "table", "pool", "q", "o"), (k, v, ints(starts(lens)), *books, q, o)):
+        g.bind(n, t)
+    g.add("store", D.to_bytes(B.kv4_store(c, sum(lens))), ["k", "v", "cu", "lens", "table", "pool"])
+    g.add("attend", D.to_bytes(B.attention_kv4(c, 8)), ["q", "lens", "table", "pool", "o"])
+    return g, o, cache_attention(q, k, v, lens, 64, 1 / math.sqrt(128))
+
+
+def test_captured_graphs_replay_on_two_streams():
+    """Two captured decode steps replayed at once share nothing; an eager run between them changes neither."""
+    (a, oa, wa), (b, ob, wb) = decode_graph(40), decode_graph(50)
+    a.capture(), b.capture()
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    oa.zero_(), ob.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        with torch.cuda.stream(sa):
+            a.cuda_graph.replay()
+        with torch.cuda.stream(sb):
+            b.cuda_graph.replay()
+    torch.cuda.synchronize()
+    near(oa, *wa, torch.bfloat16)
+    near(ob, *wb, torch.bfloat16)
+
+
+def test_launches_on_two_streams_do_not_share_a_workspace():
+    def case(seed, n):
+        c, table, pool = cache_case([n], 128, 16, 64, 1, "bfloat16", seed)
+        k, v = rows_of(n, c, seed)
+        q = torch.randn(1, 4, 128, generator=gen(seed)).to(torch.bfloat16).cuda()
+        books = [ints([n]), ints(table), pool]
+        launch(B.kv4_store(c, n), [k, v, ints([0, n])] + books)
+        return D.to_bytes(B.attention_kv4(c, 4)), [q] + books + [torch.zeros_like(q)], cache_attention(q, k, v, [n], 64, 1 / math.sqrt(128))
+    cases = [case(60, 6000), case(61, 9000)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for (blob, ts, _), s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                RC.launch_tensors(blob, ts, sync=False)
+    torch.cuda.synchronize()
+    for _, ts, want in cases:
+        near(ts[-1], *want, torch.bfloat16)
+
+
+def test_launch_tensors_can_be_captured():
+    lens = [30, 200]
+    q, k, v, q0, k0 = packed_case(lens, lens, 4, 2, 128, "bfloat16", 70)
+    o = torch.zeros_like(q)
+    a = Live()
+    blobs = [(D.to_bytes(B.attention_packed(230, 2, 4, 2)), [q, k, v, ints(q0), o]),
+             (D.to_bytes(B.pages_grow(a.c, 1)), [ints([1]), ints([20])] + a.books()),
+             (D.to_bytes(B.pages_fork(a.c, 1)), [ints([1]), ints([3])] + a.books() + [a.pool]),
+             (D.to_bytes(B.pages_free(a.c, 2)), [ints([1, 3])] + a.books())]
+    for blob, ts in blobs:
+        RC.launch_tensors(blob, ts)
+    o.zero_()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for blob, ts in blobs:
+            RC.launch_tensors(blob, ts, sync=False)
+    for _ in range(3):
+        g.replay()
+    native.sync(torch.cuda.current_stream().cuda_stream)
+    near(o, *dense(q, k, v, lens, lens, q0, k0, 1 / math.sqrt(128)), torch.bfloat16)
+    assert not a.refs.any() and not a.lens.any()
+
+
+@pytest.mark.parametrize("family", ["packed", "kv4"])
+def test_stalled_stage_times_out_and_device_stays_usable(family):
+    """A withheld copy ends in PTSIM_E_TIMEOUT within the test's limit, and the next launch is right."""
+    if family == "packed":
+        lens = [600]
+        q, k, v, q0, k0 = packed_case(lens, lens, 2, 1, 128, "bfloat16", 80)
+        o = torch.zeros_like(q)
+        desc, ts, want = B.attention_packed(600, 1, 2, 1), [q, k, v, ints(q0), o], dense(q, k, v, lens, lens, q0, k0, 1 / math.sqrt(128))
+    else:
+        lens = [900]
+        c, table, pool = cache_case(lens, 128, 16, 64, 1, "bfloat16", 81)
+        k, v = rows_of(900, c, 82)
+        q = torch.randn(1, 4, 128, generator=gen(83)).to(torch.bfloat16).cuda()
+        o, books = torch.zeros_like(q), [ints(lens), ints(table), pool]
+        launch(B.kv4_store(c, 900), [k, v, ints([0, 900])] + books)
+        desc, ts, want = B.attention_kv4(c, 4), [q] + books + [o], cache_attention(q, k, v, lens, 64, 1 / math.sqrt(128))
+    stalled = D.from_bytes(D.to_bytes(desc))
+    stalled.flags |= D.FLAG_TEST_STALL
+    assert failed(stalled, ts) == D.E_TIMEOUT
+    launch(desc, ts)
+    near(o, *want, torch.bfloat16)

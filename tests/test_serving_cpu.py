@@ -1,0 +1,197 @@
+"""The serving operators without a GPU: their descriptors and refusals (ptsim_check), their access streams, and the
+64-bit oracle's own consistency (a token written into a record reads back as the values its codes stand for)."""
+import pytest
+import torch
+
+from oracle import serving as S
+from pytorchsim_triton_compiler.codegen import build as B
+from pytorchsim_triton_compiler.codegen import descriptors as D
+from pytorchsim_triton_compiler.runtime import cuda as RC
+from pytorchsim_triton_compiler.runtime import dma_access, native
+from pytorchsim_triton_compiler.runtime.graph import Graph
+
+SHAPES = [(64, 16, 32, 2), (64, 32, 64, 1), (128, 16, 64, 2), (128, 64, 32, 1), (128, 128, 128, 1)]   # dim, page, group, hkv
+
+
+def shape(dim=128, page=16, group=64, hkv=2, slots=3, max_pages=4, pages=9, layers=2, dtype="bfloat16"):
+    return B.kv4_cache(slots=slots, max_pages=max_pages, pages=pages, hkv=hkv, dim=dim, page_size=page, group=group,
+                       layers=layers, dtype=dtype)
+
+
+def every_builder():
+    c = shape()
+    yield "packed", B.attention_packed(10, 3, 8, 2)
+    yield "packed fused", B.attention_packed(10, 3, 8, 2, 64, dtype="float16", fused=True)
+    yield "packed prefix", B.attention_packed(10, 3, 8, 2, k_tokens=21)
+    yield "packed head major", B.attention_packed(10, 3, 8, 2, head_major=True)
+    yield "store", B.kv4_store(c, 7, layer=1)
+    yield "store fused", B.kv4_store(c, 7, fused_hq=4)
+    yield "store head major", B.kv4_store(c, 7, head_major=True)
+    yield "load", B.kv4_load(c, 7)
+    yield "attention", B.attention_kv4(c, 6)
+    yield "attention fused", B.attention_kv4(c, 6, fused=True)
+    yield "grow", B.pages_grow(c, 2)
+    yield "fork", B.pages_fork(c, 2)
+    yield "copy", B.pages_fork(c, 2, deep=True)
+    yield "free", B.pages_free(c, 2)
+    yield "compact", B.pages_compact(c)
+
+
+@pytest.mark.parametrize("name,desc", list(every_builder()), ids=lambda x: x if isinstance(x, str) else "")
+def test_descriptors_validate_and_describe(name, desc):
+    blob = D.to_bytes(desc)
+    native.check(blob)
+    assert native.units(blob) == 1
+    assert D.describe(D.from_bytes(blob))["kind"] == D.KIND_NAME[desc.kind]
+    outs = RC.written_args(desc)
+    names = [f"a{i}" for i in range(desc.nargs)]
+    streams = dma_access.streams(desc, 0, 1, names)
+    assert {s["arg"] for s in streams if s["dir"] == "write"} == {names[i] for i in outs}
+    assert {s["arg"] for s in streams} == set(names)
+    for s in streams:
+        ends = dma_access.bounds(s["access"])
+        if ends is not None:
+            assert 0 <= ends[0] and ends[1] < desc.arg_numel[names.index(s["arg"])]
+
+
+def _code(desc):
+    with pytest.raises(native.ExecutorError) as e:
+        native.check(D.to_bytes(desc))
+    return e.value.code
+
+
+def _with(desc, params, **fields):
+    for k, v in fields.items():
+        setattr(getattr(desc.p, params), k, v)
+    return desc
+
+
+@pytest.mark.parametrize("fields,code", [
+    (dict(dim=96), D.E_UNSUPPORTED), (dict(hq=7), D.E_DESC), (dict(scale=0.0), D.E_UNSUPPORTED),
+    (dict(scale=float("nan")), D.E_UNSUPPORTED), (dict(scale=float("inf")), D.E_UNSUPPORTED),
+    (dict(q_tokens=11), D.E_OOB), (dict(k_tokens=11), D.E_OOB), (dict(q_off=4), D.E_UNSUPPORTED),
+    (dict(k_row=2 * 128 + 4), D.E_UNSUPPORTED), (dict(o_row=-8), D.E_DESC), (dict(seqs=4), D.E_OOB), (dict(seqs=-1), D.E_DESC),
+    (dict(seqs=D.PACKED_SEQS + 1), D.E_UNSUPPORTED), (dict(cuq_arg=0), D.E_UNSUPPORTED), (dict(o_arg=0), D.E_DESC),
+    (dict(v_arg=9), D.E_DESC), (dict(q_tokens=1 << 40), D.E_DESC)])
+def test_packed_attention_refusals(fields, code):
+    assert _code(_with(B.attention_packed(10, 3, 8, 2), "pattn", **fields)) == code
+
+
+@pytest.mark.parametrize("make", [lambda c: B.kv4_store(c, 7), lambda c: B.kv4_load(c, 7), lambda c: B.attention_kv4(c, 6)])
+@pytest.mark.parametrize("fields,code", [
+    (dict(dim=32), D.E_UNSUPPORTED), (dict(group=16), D.E_UNSUPPORTED), (dict(page_size=8), D.E_UNSUPPORTED),
+    (dict(page_size=24), D.E_UNSUPPORTED), (dict(pages=10), D.E_OOB), (dict(layers=3), D.E_OOB), (dict(layer=2), D.E_DESC),
+    (dict(layer=-1), D.E_DESC), (dict(slots=4), D.E_OOB), (dict(slots=D.KV4_SLOTS + 1), D.E_UNSUPPORTED),
+    (dict(max_pages=5), D.E_OOB), (dict(max_pages=1 << 40), D.E_DESC), (dict(hkv=0), D.E_DESC), (dict(a_off=1), D.E_UNSUPPORTED),
+    (dict(a_off=1 << 20), D.E_OOB), (dict(b_row=12), D.E_UNSUPPORTED), (dict(pool_arg=-1), D.E_DESC), (dict(lens_arg=99), D.E_DESC)])
+def test_cache_refusals(make, fields, code):
+    assert _code(_with(make(shape()), "kv4", **fields)) == code
+
+
+def test_cache_refusals_of_types():
+    d = B.attention_kv4(shape(), 6)
+    d.arg_dtype[0] = D.DTYPE_CODE["float32"]
+    assert _code(d) == D.E_UNSUPPORTED
+    d = B.attention_kv4(shape(), 6)
+    d.arg_dtype[d.p.kv4.b_arg] = D.DTYPE_CODE["float16"]      # q and o of two types
+    assert _code(d) == D.E_UNSUPPORTED
+    assert _code(_with(B.attention_kv4(shape(), 6), "kv4", hq=5)) == D.E_DESC
+    assert _code(_with(B.attention_kv4(shape(), 6), "kv4", scale=-1.0)) == D.E_UNSUPPORTED
+    d = B.kv4_store(shape(), 7)
+    d.units = 2
+    assert _code(d) == D.E_DESC
+    for bad in (dict(dim=96), dict(page_size=48), dict(group=128, dim=64)):
+        with pytest.raises(ValueError):
+            B.kv4_cache(slots=1, max_pages=1, pages=1, hkv=1, **bad)
+
+
+@pytest.mark.parametrize("make,fields,code", [
+    (lambda c: B.pages_grow(c, 2), dict(op=9), D.E_DESC), (lambda c: B.pages_grow(c, 2), dict(n=3), D.E_OOB),
+    (lambda c: B.pages_grow(c, 2), dict(n=D.PAGES_IDS + 1), D.E_UNSUPPORTED), (lambda c: B.pages_grow(c, 2), dict(n=-1), D.E_DESC),
+    (lambda c: B.pages_grow(c, 2), dict(pages=10), D.E_OOB), (lambda c: B.pages_grow(c, 2), dict(slots=0, n=2), D.E_DESC),
+    (lambda c: B.pages_grow(c, 2), dict(page_size=0), D.E_DESC), (lambda c: B.pages_grow(c, 2), dict(aux_arg=-1), D.E_DESC),
+    (lambda c: B.pages_fork(c, 2), dict(pool_arg=-1), D.E_DESC), (lambda c: B.pages_fork(c, 2), dict(layers=3), D.E_OOB),
+    (lambda c: B.pages_fork(c, 2), dict(page_bytes=24), D.E_DESC), (lambda c: B.pages_free(c, 2), dict(max_pages=5), D.E_OOB),
+    (lambda c: B.pages_compact(c), dict(n=1), D.E_DESC), (lambda c: B.pages_compact(c), dict(pool_arg=0), D.E_UNSUPPORTED)])
+def test_page_refusals(make, fields, code):
+    assert _code(_with(make(shape()), "pages", **fields)) == code
+
+
+def test_launches_refuse_a_small_workspace_and_null_pointers_before_any_gpu():
+    assert native.workspace_size(D.to_bytes(B.attention_kv4(shape(), 6))) > 0
+    assert native.workspace_size(D.to_bytes(B.pages_fork(shape(), 2))) == 4 * (4 + 3 * 9)
+    assert native.workspace_size(D.to_bytes(B.pages_free(shape(), 2))) == 0
+    blob = D.to_bytes(B.pages_compact(shape()))
+    with pytest.raises(native.ExecutorError) as e:
+        native.launch(blob, [0, 1, 1, 1], 0, 1)
+    assert e.value.code == D.E_ARGS
+
+
+def test_builders_refuse_a_fused_projection_with_another_layout():
+    for make in (lambda: B.attention_packed(8, 1, 4, 2, fused=True, head_major=True),
+                 lambda: B.attention_packed(8, 1, 4, 2, fused=True, k_tokens=9),
+                 lambda: B.kv4_store(shape(), 7, fused_hq=4, head_major=True)):
+        with pytest.raises(ValueError):
+            make()
+
+
+def test_graph_binds_device_tensors_only():
+    g = Graph("cuda:0")
+    with pytest.raises(ValueError):
+        g.bind("x", torch.zeros(4))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_quantisation_is_within_its_step(dtype, group):
+    x = (torch.randn(50, 128, generator=torch.Generator().manual_seed(1)) * 3 + 1).to(dtype)
+    x[0] = 2.5                                       # constant: exact
+    x[1, :] = torch.tensor([-60000.0, 60000.0]).to(dtype).repeat(64)   # a range no sum of two can hold in fp16
+    code, scale, mn = S.quantise(x, group)
+    back = S.dequantised(x, group)
+    assert torch.equal(back[0], x[0].double())
+    assert int(code.min()) >= 0 and int(code.max()) == 15
+    # Rounding: half a step; the rounded scale moves code 15 by 15 half units in the last place of the scale, the clamp by no more.
+    step = scale.double().repeat_interleave(group, -1)
+    assert bool(((back - x.double()).abs() <= step * (0.5 + 15 * torch.finfo(dtype).eps / 2) * (1 + 1e-6) + 1e-30).all())
+
+
+def test_a_group_with_a_non_finite_value_stands_for_nan():
+    x = torch.randn(3, 128, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    x[0, 3], x[1, 70], x[2, 0] = float("nan"), float("inf"), -float("inf")
+    bad = torch.isnan(S.dequantised(x, 64))
+    assert bad[0, :64].all() and not bad[0, 64:].any() and bad[1, 64:].all() and not bad[1, :64].any() and bad[2, :64].all()
+
+
+@pytest.mark.parametrize("dim,page,group,hkv", SHAPES)
+def test_records_hold_what_was_written(dim, page, group, hkv):
+    c = shape(dim, page, group, hkv, slots=1, max_pages=2, pages=3)
+    cache = S.Cache(c, torch.zeros(c.pool_bytes, dtype=torch.uint8), [[2, 0]], [page + 3])
+    assert cache.pool.shape[-1] * hkv == c.page_bytes
+    gen = torch.Generator().manual_seed(dim + page)
+    k, v = (torch.randn(page + 3, hkv, dim, generator=gen).to(torch.bfloat16) for _ in "kv")
+    for t in range(page + 3):
+        for h in range(hkv):
+            cache.write(0, t, h, k[t, h], v[t, h], layer=1)
+    for t in range(page + 3):
+        for h in range(hkv):
+            a, b = cache.read(0, t, h, layer=1)
+            assert torch.equal(a, S.dequantised(k[t, h], group)) and torch.equal(b, S.dequantised(v[t, h], group))
+    # Every byte of a full record belongs to one token, K or V, code or parameter.
+    seen = set()
+    for kk, vv, kp, vp in cache.where:
+        seen |= {b for b, _ in kk} | {b for b, _ in vv} | {p + i for p in kp + vp for i in range(4)}
+    assert seen == set(range(c.page_bytes // hkv))
+
+
+def test_page_oracle_forks_frees_and_compacts():
+    pool = torch.arange(2 * 8 * 4).view(2, 8, 4)
+    p = S.Pages([[-1] * 3 for _ in range(3)], [0, 0, 0], [0] * 8, pool, 4)
+    p.grow([0, 1], [9, 4])
+    assert p.table == [[0, 1, 2], [3, -1, -1], [-1] * 3] and p.refs == [1, 1, 1, 1, 0, 0, 0, 0]
+    p.fork([0], [2])
+    assert p.table[2] == [0, 1, 4] and p.refs == [2, 2, 1, 1, 1, 0, 0, 0] and torch.equal(p.pool[:, 4], p.pool[:, 2])
+    p.free([1, 0])
+    assert p.table[:2] == [[-1] * 3] * 2 and p.refs == [1, 1, 0, 0, 1, 0, 0, 0]
+    p.compact()
+    assert p.table[2] == [0, 1, 2] and p.refs == [1, 1, 1, 0, 0, 0, 0, 0]
