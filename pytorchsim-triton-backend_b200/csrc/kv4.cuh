@@ -1,14 +1,17 @@
 // The 4-bit paged cache of keys and values (format: include/ptsim_b200.h, ptsim_kv4_params): store, load and the attention
 // of one new token per slot.  No counterpart in the reference, whose decode program reads a dense bf16 cache (decode.cuh).
 //
-// Attention.  With codes c, scale a and minimum b per (key, group of the head dimension), the cached key is k = a c + b and
-// the score z = sum_g a_g (q . c)_g + b_g sum(q)_g: the tensor core multiplies q by the small integers c, exact in 16 bits, and
-// the parameters enter in fp32, once per (key, group).  Likewise O = sum_k (p a_g) (c - 8) + p (b_g + 8 a_g), with p a_g
-// rounded to 16 bits as the product's operand (the rounding of P that decode.cuh makes, here of what multiplies |c - 8| <= 8)
-// and the second sum kept per row in fp32.  A nibble becomes a 16-bit float by one mask-and-or, bf16 0x4300 | c = 128 + c and
-// fp16 0x5400 | c << 4 = 64 + c.  For K the offset's share of a score, 128 sum(q), is taken off in the accumulator's start.
-// For V it is subtracted from the operand: accumulated over 10^5 keys, an offset of 128 costs the sums their low bits
-// (the tensor core truncates; measured 2.4e-2 of the result at 131072 keys against 1.7e-3 with c - 8).
+// Attention.  With codes c, scale a and minimum b per (key, group of the head dimension), the cached key is a c + b =
+// a (c - 8) + (b + 8 a) and the score z = sum_g a_g (q . (c - 8))_g + (b_g + 8 a_g) sum(q)_g: the tensor core multiplies q by
+// small integers, exact in 16 bits, and the parameters enter in fp32, once per (key, group).  Likewise
+// O = sum_k (p a_g) (c - 8) + p (b_g + 8 a_g), with p a_g rounded to fp16 as the product's operand (2^-12 of what multiplies
+// |c - 8| <= 8) and the second sum kept per row in fp32.  Both products run in fp16 whatever the cache's type: a byte of two
+// codes becomes two fp16 operands by half a byte permute (0x64 above the byte: 1024 + lo + 16 hi), one mask-and-or
+// (1032 + 16 hi), one subtraction (lo - 8) and one fused multiply-add (hi - 8), two of them on the FMA pipe; bf16, with 7 bits
+// of mantissa, takes a shift more per pair, all on the half-rate ALU pipe, which bounded that form (63 % busy, 467 warp
+// instructions per 16 keys, 166 us at 4 slots of up to 131072 keys).  bf16 queries fit fp16 after division by their row's power of
+// two; the weights' V scales by a power of two that follows the largest scale seen.  The operands are centred because a
+// constant offset costs the sums their low bits: with 128 + c for V, 10^5 keys ended 2.4e-2 off (the tensor core truncates).
 //
 // The products have K and V as the 16-row operand: S^T = K q^T, O^T = V^T P^T (mma.sync m16n8k16, N = 8 query rows of one KV
 // head), so up to 8 query heads per KV head waste nothing, half of what a 16-row query tile costs; tcgen05.mma, whose
@@ -16,12 +19,12 @@
 // take their k index in any order both sides agree on, which the page format uses: 16-byte (K) and 8-byte (V) shared loads
 // without bank conflicts give words whose nibbles are the fragments.
 //
-// Bound: HBM, (D + 8 D / group) bytes per key and KV head (144 at D 128, group 64: 3.5 times fewer than bf16), and close
-// behind it the issue slots of the unpacking (about 250 warp instructions per 16 keys).  Work is one list of 32-key tiles over
-// (slot, KV head), cut into equal contiguous ranges, one per warp: a warp streams its tiles by bulk copies through a ring of its
-// own (no barrier between warps) and keeps the online softmax in registers.  Lengths are read on the device, so any
-// raggedness is balanced to a tile.  A range that holds only part of an item leaves (m, l, O) in the workspace and a second
-// kernel (a programmatic dependent) merges the parts in key order: results do not depend on timing.
+// Bound: HBM, (D + 8 D / group) bytes per key and KV head (144 at D 128, group 64: 3.5 times fewer than bf16), and before
+// it the issue slots of the unpacking.  Work is one list of 32-key tiles over (slot, KV head), cut into equal contiguous
+// ranges, one per warp: a warp streams its tiles by bulk copies through a ring of its own (no barrier between warps) and keeps
+// the online softmax in registers.  Lengths are read on the device, so any raggedness is balanced to a tile.  A range that
+// holds only part of an item leaves (m, l, O) in the workspace and a second kernel (a programmatic dependent) merges the parts
+// in key order: results do not depend on timing.
 #pragma once
 #include "sm100.cuh"
 #include "decode.cuh"
@@ -40,9 +43,10 @@ struct Kv4Args {
   int64_t a_row, a_head, b_row, b_head;
   int64_t record;                    // bytes of one (page, KV head)
   int32_t tokens, slots, hkv, per, rb;   // per: query heads of a KV head; rb: blocks of 16 of them
-  int32_t pages, page_size, max_pages;
+  int32_t pages, page_size, page_log, max_pages;
   float sl;                          // scale * log2 e
   float *part_o, *part_ml;           // [2 * workers][16][D] and [2 * workers][16][2]
+  int32_t *before;                   // [slots + 1] tiles before a slot, for the merge
   int32_t workers, stall;
 };
 
@@ -228,41 +232,25 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const __grid_constant__ K
 // -------------------------------------------------------------------------------------------------------------------
 // Attention
 // -------------------------------------------------------------------------------------------------------------------
-template <bool F16>
-__device__ __forceinline__ void mma_16n8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  if (F16)
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  else
-    mma_16816(d, a, b0, b1);
+__device__ __forceinline__ void mma_16n8_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Nibbles j and 4 + j of w as a pair of 16-bit floats kOff + code.
-template <bool F16, int J>
-__device__ __forceinline__ uint32_t nibbles(uint32_t w) {
-  if (F16) {
-    const uint32_t s = J == 0 ? w << 4 : w >> (4 * (J > 0 ? J - 1 : 0));
-    return (s & 0x00f000f0u) | 0x54005400u;
-  }
-  return ((w >> (4 * J)) & 0x000f000fu) | 0x43004300u;
+// x = a pair of fp16 1024 + lo + 16 hi (codes lo, hi of a byte): the pairs lo - 8 and hi - 8, exact.
+__device__ __forceinline__ void split_codes(uint32_t x, uint32_t &lo, uint32_t &hi) {
+  const uint32_t y = (x & 0xfff0fff0u) | 0x00080008u;                                    // 1032 + 16 hi
+  asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(y));
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(hi) : "r"(y), "r"(0x2c002c00u), "r"(0xd488d488u));   // y / 16 - 72.5
 }
-// The same less kOff + 8: code - 8, exact.
-template <bool F16, int J>
-__device__ __forceinline__ uint32_t centred(uint32_t w) {
-  uint32_t r;
-  const uint32_t x = nibbles<F16, J>(w);
-  if (F16) asm("sub.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x54805480u));
-  else asm("sub.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x43084308u));
-  return r;
-}
-template <bool F16>
-constexpr float kKvOff = F16 ? 64.0f : 128.0f;
 
-// How far (log2) a score may pass its row's reference before the reference moves.  The weight times the V scale is an operand
-// in the cache's type: fp16 holds 2^2 times the largest scale of fp16 values, (2 * 65504) / 15, and no 2^3.
+// How far (log2) a score may pass its row's reference before the reference moves.  The weight times the V scale is an fp16
+// operand: fp16 caches have scales up to 2 * 65504 / 15, and fp16 holds 2^2 times that, no 2^3; bf16 caches' scales are divided
+// by a power of two that keeps them to 2^6 (kKvScaleRoom), so that 2^14 bounds the product.
 template <bool F16>
 constexpr float kKvGrow = F16 ? 2.0f : 8.0f;
+constexpr int kKvScaleRoom = 6;
 
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t r;
@@ -289,7 +277,6 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
   constexpr int kStage = kKvTile * (D + 8 * NG);            // bytes of a tile: one block of 32 keys or two of 16
   constexpr int kWordsK = D / 32, kWordsV = D / 64;         // words a lane takes of a K and of a V row
   constexpr int kGroup = D / NG;
-  constexpr float kOff = kKvOff<F16>;
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t *ring = smem + (threadIdx.x >> 5) * kKvStages * kStage;
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + kKvWarps * kKvStages * kStage) + (threadIdx.x >> 5) * kKvStages;
@@ -324,6 +311,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
   }
   if (threadIdx.x == kKvWarps * 32 - 1) before[g.slots] = scan;
   __syncthreads();
+  if (blockIdx.x == 0)
+    for (int s = threadIdx.x; s <= g.slots; s += kKvWarps * 32) g.before[s] = before[s];
 
   const int items = g.hkv * g.rb;                           // items of a slot
   const int64_t total = int64_t(before[g.slots]) * items;
@@ -332,9 +321,9 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
   if (worker >= n) return;
   const int64_t w_lo = kv4_start(worker, total, n), w_hi = kv4_start(worker + 1, total, n);
 
-  // Position in the list: slot, item of the slot, tile of the item.
+  // Position in the list: slot, its length and tiles, KV head and row block, tile of the item.
   struct Cursor {
-    int slot, item, tile, tiles;
+    int slot, len, tiles, head, block, tile;
   };
   auto seek = [&](int64_t x) {
     int lo = 0, hi = g.slots;                               // the last slot with before * items <= x
@@ -345,63 +334,65 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
     }
     Cursor c;
     c.slot = lo;
+    c.len = g.lens[lo];
     c.tiles = before[lo + 1] - before[lo];
-    const int64_t in = x - int64_t(before[lo]) * items;
-    c.item = int(in / c.tiles);
-    c.tile = int(in % c.tiles);
+    const uint32_t in = uint32_t(x - int64_t(before[lo]) * items), item = in / uint32_t(c.tiles);
+    c.head = int(item) / g.rb;
+    c.block = int(item) % g.rb;
+    c.tile = int(in % uint32_t(c.tiles));
     return c;
   };
-  auto step = [&](Cursor &c) {
-    if (++c.tile < c.tiles) return;
+  auto next_item = [&](Cursor &c) {
     c.tile = 0;
-    if (++c.item < items) return;
-    c.item = 0;
+    if (++c.block < g.rb) return;
+    c.block = 0;
+    if (++c.head < g.hkv) return;
+    c.head = 0;
     do {
       ++c.slot;
       c.tiles = c.slot < g.slots ? before[c.slot + 1] - before[c.slot] : 1;
     } while (c.tiles == 0);
+    c.len = c.slot < g.slots ? g.lens[c.slot] : 0;
   };
 
   // Producer side: lane k < parts holds the pool page of the k-th part of the tile that is copied next.
-  const int bs = g.page_size < kKvTile ? g.page_size : kKvTile, parts = kKvTile / bs;
+  const int bs_log = min(g.page_log, 5), bs = 1 << bs_log, parts = kKvTile >> bs_log;
   const uint32_t part_bytes = uint32_t(bs * (D + 8 * NG));
-  auto next_page = [&](const Cursor &c, bool any) {
+  auto next_page = [&](const Cursor &c) {
     int page = -2;                                          // -2: no key of the slot lies there
-    if (any && lane < parts) {
-      const int first = c.tile * kKvTile + lane * bs;
-      if (first < g.lens[c.slot]) {
-        page = g.table[int64_t(c.slot) * g.max_pages + first / g.page_size];
-        if (page < 0 || page >= g.pages) page = -1;
-      }
+    const int first = c.tile * kKvTile + lane * bs;
+    if (lane < parts && first < c.len) {
+      page = g.table[int64_t(c.slot) * g.max_pages + (first >> g.page_log)];
+      if (page < 0 || page >= g.pages) page = -1;
     }
     return page;
   };
-  auto copy = [&](const Cursor &c, int page, int64_t x) {
-    const int st = int(x - w_lo) % kKvStages;
+  int fill_st = 0;
+  auto copy = [&](const Cursor &c, int page, bool withheld) {
     const uint32_t ok = __ballot_sync(0xffffffffu, page >= 0);
     if (lane < parts && page == -1) record_status(PTSIM_E_OOB);
     if (lane == 0) {
-      good[st] = int(ok);
-      sm100::mbar_arrive_expect_tx(&full[st], part_bytes * __popc(ok));
+      good[fill_st] = int(ok);
+      sm100::mbar_arrive_expect_tx(&full[fill_st], part_bytes * __popc(ok));
     }
     __syncwarp();
-    if (page >= 0 && !(g.stall && blockIdx.x == 0 && warp == 0 && x == w_lo)) {   // test hook: armed, no copy in flight
-      const int block = ((c.tile * kKvTile + lane * bs) & (g.page_size - 1)) / bs;
-      const uint8_t *src = g.pool + (int64_t(page) * g.hkv + c.item / g.rb) * g.record + uint32_t(block) * part_bytes;
-      sm100::bulk_load_g2s(ring + st * kStage + lane * part_bytes, src, part_bytes, &full[st]);
+    if (page >= 0 && !withheld) {
+      const int block = ((c.tile * kKvTile + lane * bs) & ((1 << g.page_log) - 1)) >> bs_log;
+      const uint8_t *src = g.pool + (int64_t(page) * g.hkv + c.head) * g.record + uint32_t(block) * part_bytes;
+      sm100::bulk_load_g2s(ring + fill_st * kStage + lane * part_bytes, src, part_bytes, &full[fill_st]);
     }
+    fill_st = fill_st + 1 == kKvStages ? 0 : fill_st + 1;
   };
 
   Cursor use = seek(w_lo), fill = use;
-  int64_t fx = w_lo;                                        // next tile to copy
-  int page = next_page(fill, true);
-  auto feed = [&]() {                                       // copy tile fx, then fetch the next one's pages
-    if (fx >= w_hi) return;
-    copy(fill, page, fx);
-    ++fx;
-    if (fx < w_hi) {
-      step(fill);
-      page = next_page(fill, true);
+  const int count = int(w_hi - w_lo);
+  int filled = 0, page = next_page(fill);
+  auto feed = [&]() {                                       // copy the next tile, then fetch the pages of the one after it
+    if (filled >= count) return;
+    copy(fill, page, g.stall && blockIdx.x == 0 && warp == 0 && filled == 0);   // test hook: armed, no copy in flight
+    if (++filled < count) {
+      if (++fill.tile == fill.tiles) next_item(fill);
+      page = next_page(fill);
     }
   };
   for (int i = 0; i < kKvStages; ++i) feed();
@@ -409,34 +400,54 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
   // Offsets of a 16-key step within a tile.
   const bool small = bs == 16;
   const int step_k = small ? 16 * (D + 8 * NG) : 8 * D, step_p = small ? 16 * (D + 8 * NG) : 64 * NG;
-  const int v_at = bs * (D / 2), kp_at = bs * D, vp_at = kp_at + bs * 4 * NG;
-  const int v_lane = qd * (D / 2) + (D == 128 ? (gq ^ ((qd & 2) << 1)) * 8 : gq * 4);
+  const int v_at = bs * (D / 2) + qd * (D / 2) + (D == 128 ? (gq ^ ((qd & 2) << 1)) * 8 : gq * 4);
+  const int kp_at = bs * D + gq * NG * 4, vp_at = kp_at + bs * 4 * NG;
 
   bool ok = true;
-  int64_t x = w_lo;
-  while (ok && x < w_hi) {
+  int done = 0, st = 0, phase = 0;
+  while (done < count) {
     // One item's part: tiles [use.tile, last) of (slot, KV head, row block).
-    const int slot = use.slot, head = use.item / g.rb, row0 = (use.item % g.rb) * 16;
-    const int first = use.tile, last = int(min(int64_t(use.tiles), use.tile + (w_hi - x)));
-    const int rows = min(16, g.per - row0), len = g.lens[slot];
-    const bool whole = first == 0 && last == use.tiles, opening = x == w_lo;
+    const int slot = use.slot, head = use.head, row0 = use.block * 16, len = use.len;
+    const int first = use.tile, last = min(use.tiles, use.tile + count - done);
+    const int rows = min(16, g.per - row0);
+    const bool whole = first == 0 && last == use.tiles, opening = done == 0;
 
-    uint32_t qb[NT][kWordsK][4];                            // d = 32 b + 8 qd + 0 .. 7 of row gq
-    float qsum[NT][2][NG];                                  // of rows 2 qd and 2 qd + 1, per group
+    uint32_t qb[NT][kWordsK][4];                            // fp16 pairs of d = 32 b + 8 qd + 0 .. 7 of row gq
+    float qsum[NT][2][NG], sl[NT][2];                       // of rows 2 qd and 2 qd + 1: sums per group, scale
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int r = t * 8 + gq;
       const uint16_t *q = g.a + slot * g.a_row + int64_t(head * g.per + row0 + r) * g.a_head + qd * 8;
-      float s[NG];
+      float s[NG], back = g.sl;
 #pragma unroll
       for (int i = 0; i < NG; ++i) s[i] = 0.f;
 #pragma unroll
       for (int b = 0; b < kWordsK; ++b) {
         const uint4 w = r < rows ? *reinterpret_cast<const uint4 *>(q + b * 32) : make_uint4(0, 0, 0, 0);
         qb[t][b][0] = w.x, qb[t][b][1] = w.y, qb[t][b][2] = w.z, qb[t][b][3] = w.w;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[b * 32 / kGroup] += lo_f32<F16>(qb[t][b][i]) + hi_f32<F16>(qb[t][b][i]);
       }
+      if (!F16) {
+        // bf16 to fp16: divided by the power of two of the row's largest value, whose 8 bits fp16's 11 hold; values 2^-14 of it
+        // and less keep 2^-25 of it.  A row of zeros, or with an infinity or a NaN, is converted as it is.
+        uint32_t top = 0;
+#pragma unroll
+        for (int b = 0; b < kWordsK; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) top = max(top, max((qb[t][b][i] >> 7) & 0xffu, (qb[t][b][i] >> 23) & 0xffu));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = top == 0 || top == 255 ? 0 : int(top) - 127;
+        const float down = __uint_as_float(uint32_t(127 - (e > 126 ? 126 : e)) << 23);
+        back = g.sl / down;
+#pragma unroll
+        for (int b = 0; b < kWordsK; ++b)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) qb[t][b][i] = pack_16x2<true>(lo_bf16(qb[t][b][i]) * down, hi_bf16(qb[t][b][i]) * down);
+      }
+#pragma unroll
+      for (int b = 0; b < kWordsK; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[b * 32 / kGroup] += lo_f32<true>(qb[t][b][i]) + hi_f32<true>(qb[t][b][i]);
 #pragma unroll
       for (int i = 0; i < NG; ++i) {
         s[i] += __shfl_xor_sync(0xffffffffu, s[i], 1);
@@ -444,14 +455,19 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
         qsum[t][0][i] = __shfl_sync(0xffffffffu, s[i], 8 * qd);
         qsum[t][1][i] = __shfl_sync(0xffffffffu, s[i], 8 * qd + 4);
       }
+      sl[t][0] = __shfl_sync(0xffffffffu, back, 8 * qd);
+      sl[t][1] = __shfl_sync(0xffffffffu, back, 8 * qd + 4);
     }
-    float m[NT][2], l[NT][2], corr[NT][2][NG], o[NT][D / 16][4];
+    // m: the rows' references (log2), 0 until a score has been seen (seen < 0: none); room: the score that moves it.
+    float m[NT][2], room[NT][2], l[NT][2], corr[NT][2][NG], o[NT][D / 16][4];
+    float vdown = 1.f;                                      // power of two on the V scales (bf16 caches)
+    uint32_t vroom = 0;                                     // largest V scale (bits) it allows
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        m[t][i] = -INFINITY;
-        l[t][i] = 0.f;
+        m[t][i] = l[t][i] = 0.f;
+        room[t][i] = -INFINITY;
 #pragma unroll
         for (int k = 0; k < NG; ++k) corr[t][i][k] = 0.f;
       }
@@ -459,9 +475,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
       for (int i = 0; i < D / 16; ++i) o[t][i][0] = o[t][i][1] = o[t][i][2] = o[t][i][3] = 0.f;
     }
 
-    for (int tile = first; tile < last; ++tile, ++x) {
-      const int st = int(x - w_lo) % kKvStages;
-      if (!sm100::mbar_wait(&full[st], uint32_t(int(x - w_lo) / kKvStages) & 1, wl)) {
+    for (int tile = first; tile < last; ++tile) {
+      if (!sm100::mbar_wait(&full[st], phase, wl)) {
         ok = false;
         break;
       }
@@ -483,8 +498,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
           *reinterpret_cast<uint2 *>(wa) = *reinterpret_cast<const uint2 *>(kc);
           *reinterpret_cast<uint2 *>(wb) = *reinterpret_cast<const uint2 *>(kc + 8 * (D / 2));
         }
-        const uint32_t *kpar = reinterpret_cast<const uint32_t *>(buf + kp_at + h * step_p) + gq * NG;
-        const uint32_t *vpar = reinterpret_cast<const uint32_t *>(buf + vp_at + h * step_p) + gq * NG;
+        const uint32_t *kpar = reinterpret_cast<const uint32_t *>(buf + kp_at + h * step_p);
+        const uint32_t *vpar = reinterpret_cast<const uint32_t *>(buf + vp_at + h * step_p);
 #pragma unroll
         for (int i = 0; i < NG; ++i) {
           kp[0][i] = kpar[i], kp[1][i] = kpar[8 * NG + i];
@@ -494,30 +509,34 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = 0; i < NG; ++i) {
-            acc[t][i][0] = acc[t][i][2] = -kOff * qsum[t][0][i];
-            acc[t][i][1] = acc[t][i][3] = -kOff * qsum[t][1][i];
+          for (int i = 0; i < NG; ++i) acc[t][i][0] = acc[t][i][1] = acc[t][i][2] = acc[t][i][3] = 0.f;
+#pragma unroll
+        for (int b = 0; b < kWordsK; ++b)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {                     // bytes 0 and 2: d = 0, 1 | 2, 3; bytes 1 and 3: 4, 5 | 6, 7
+            uint32_t a[4];
+            split_codes(__byte_perm(wa[b], 0x64646464u, e ? 0x4341 : 0x4240), a[0], a[2]);
+            split_codes(__byte_perm(wb[b], 0x64646464u, e ? 0x4341 : 0x4240), a[1], a[3]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma_16n8_f16(acc[t][b * 32 / kGroup], a, qb[t][b][2 * e], qb[t][b][2 * e + 1]);
           }
 #pragma unroll
-        for (int b = 0; b < kWordsK; ++b) {
-          const uint32_t a0[4] = {nibbles<F16, 0>(wa[b]), nibbles<F16, 0>(wb[b]), nibbles<F16, 1>(wa[b]), nibbles<F16, 1>(wb[b])};
-          const uint32_t a1[4] = {nibbles<F16, 2>(wa[b]), nibbles<F16, 2>(wb[b]), nibbles<F16, 3>(wa[b]), nibbles<F16, 3>(wb[b])};
+        for (int k = 0; k < 2; ++k) {
+          float a[NG], mid[NG];
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            mma_16n8<F16>(acc[t][b * 32 / kGroup], a0, qb[t][b][0], qb[t][b][1]);
-            mma_16n8<F16>(acc[t][b * 32 / kGroup], a1, qb[t][b][2], qb[t][b][3]);
-          }
+          for (int i = 0; i < NG; ++i) a[i] = lo_f32<F16>(kp[k][i]), mid[i] = fmaf(8.f, a[i], hi_f32<F16>(kp[k][i]));
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              float s = mid[0] * qsum[t][i][0];
+#pragma unroll
+              for (int n = 1; n < NG; ++n) s = fmaf(mid[n], qsum[t][i][n], s);
+#pragma unroll
+              for (int n = 0; n < NG; ++n) s = fmaf(a[n], acc[t][n][2 * k + i], s);
+              z[h][t][2 * k + i] = s * sl[t][i];
+            }
         }
-#pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            float s = 0.f;
-#pragma unroll
-            for (int i = 0; i < NG; ++i)
-              s = fmaf(lo_f32<F16>(kp[k >> 1][i]), acc[t][i][k], fmaf(hi_f32<F16>(kp[k >> 1][i]), qsum[t][k & 1][i], s));
-            z[h][t][k] = s * g.sl;
-          }
         if (partial) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
@@ -530,13 +549,43 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
           }
         }
       }
-      // A row's reference moves only when a score passes it by kKvGrow (the first key always does).
+      // A row's reference moves only when a score passes it by kKvGrow (the first key's always does).
       bool grow = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) grow |= z[k >> 2][t][k & 3] > m[t][k & 1] + kKvGrow<F16>;
+        for (int i = 0; i < 2; ++i)
+          grow |= fmaxf(fmaxf(z[0][t][i], z[0][t][i + 2]), fmaxf(z[1][t][i], z[1][t][i + 2])) > room[t][i];
+      uint32_t vtop = 0;
+      if (!F16) {
+        vtop = vp[0][0][0];
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) vtop = __vmaxu2(vtop, vp[k >> 1][k & 1][i]);
+        vtop &= 0xffffu;
+        grow |= vtop > vroom;
+      }
       if (__any_sync(0xffffffffu, grow)) {
+        float f = 1.f;                                      // the V scales' power of two moves down
+        if (!F16) {
+          uint32_t top = 0;                                 // the largest finite scale
+#pragma unroll
+          for (int i = 0; i < NG; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t a = vp[k >> 1][k & 1][i] & 0xffffu;
+              if (a < 0x7f80u) top = max(top, a);
+            }
+          top = __reduce_max_sync(0xffffffffu, top);
+          if (top > vroom) {
+            const int e = min(max(int(top >> 7) - 126, -125), 126);            // 2^e > the scale
+            const float now = __uint_as_float(uint32_t(127 - e) << 23);
+            f = vroom == 0 ? 1.f : now / vdown;
+            vdown = now;
+            vroom = uint32_t(min(e + kKvScaleRoom + 127, 254)) << 7;
+          }
+        }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -544,12 +593,16 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
             float top = fmaxf(fmaxf(z[0][t][i], z[0][t][i + 2]), fmaxf(z[1][t][i], z[1][t][i + 2]));
 #pragma unroll
             for (int s = 4; s < 32; s *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
-            const float to = fmaxf(m[t][i], top);
-            const float alpha = to == m[t][i] ? 1.f : ex2_fast(m[t][i] - to);   // equal: both may be -inf
-            m[t][i] = to;
+            float alpha = 1.f;
+            if (top > room[t][i] - kKvGrow<F16>) {          // past the reference, or the first score: nothing to rescale then
+              if (room[t][i] != -INFINITY) alpha = ex2_fast(m[t][i] - top);
+              m[t][i] = top;
+              room[t][i] = top + kKvGrow<F16>;
+            }
             l[t][i] *= alpha;
 #pragma unroll
             for (int k = 0; k < NG; ++k) corr[t][i][k] *= alpha;
+            alpha *= f;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) o[t][k][i] *= alpha, o[t][k][i + 2] *= alpha;
           }
@@ -559,25 +612,27 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
         // Weights times the V scales, rounded: per group the operand [16 keys x 8 rows], transposed from the scores' layout.
         uint32_t pb[NT][NG][2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          float p[4];
+        for (int k = 0; k < 2; ++k) {
+          float a[NG], mid[NG];
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            p[k] = ex2_fast(z[h][t][k] - (m[t][k & 1] == -INFINITY ? 0.f : m[t][k & 1]));
-            l[t][k & 1] += p[k];
+          for (int i = 0; i < NG; ++i) {
+            a[i] = lo_f32<F16>(vp[h][k][i]), mid[i] = fmaf(8.f, a[i], hi_f32<F16>(vp[h][k][i]));
+            if (!F16) a[i] *= vdown;
           }
 #pragma unroll
-          for (int i = 0; i < NG; ++i)
+          for (int t = 0; t < NT; ++t) {
+            const float p0 = ex2_fast(z[h][t][2 * k] - m[t][0]), p1 = ex2_fast(z[h][t][2 * k + 1] - m[t][1]);
+            l[t][0] += p0;
+            l[t][1] += p1;
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float a = lo_f32<F16>(vp[h][k][i]), mid = fmaf(8.f, a, hi_f32<F16>(vp[h][k][i]));
-              const uint32_t w = pack_16x2<F16>(p[2 * k] * a, p[2 * k + 1] * a);
-              corr[t][0][i] = fmaf(p[2 * k], mid, corr[t][0][i]);
-              corr[t][1][i] = fmaf(p[2 * k + 1], mid, corr[t][1][i]);
-              pb[t][i][k] = transpose_8x8(w);
+            for (int i = 0; i < NG; ++i) {
+              corr[t][0][i] = fmaf(p0, mid[i], corr[t][0][i]);
+              corr[t][1][i] = fmaf(p1, mid[i], corr[t][1][i]);
+              pb[t][i][k] = transpose_8x8(pack_16x2<true>(p0 * a[i], p1 * a[i]));
             }
+          }
         }
-        const uint8_t *vc = buf + v_at + h * step_k + v_lane;   // keys 2 qd, 2 qd + 1, 2 qd + 8, 2 qd + 9: rows qd, + 4, + 8, + 12
+        const uint8_t *vc = buf + v_at + h * step_k;            // keys 2 qd, 2 qd + 1, 2 qd + 8, 2 qd + 9: rows qd, + 4, + 8, + 12
         __align__(8) uint32_t w[4][kWordsV];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -587,26 +642,31 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
 #pragma unroll
         for (int v = 0; v < kWordsV; ++v)
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {                // nibbles 0-3: d = 64 v + 4 gq ..; 4-7: 32 further
-            const uint32_t lo = __byte_perm(w[0][v], w[1][v], half ? 0x7632 : 0x5410);
-            const uint32_t hi = __byte_perm(w[2][v], w[3][v], half ? 0x7632 : 0x5410);
-            const uint32_t a0[4] = {centred<F16, 0>(lo), centred<F16, 1>(lo), centred<F16, 0>(hi), centred<F16, 1>(hi)};
-            const uint32_t a1[4] = {centred<F16, 2>(lo), centred<F16, 3>(lo), centred<F16, 2>(hi), centred<F16, 3>(hi)};
+          for (int half = 0; half < 2; ++half) {                // bytes 0, 1: d = 64 v + 4 gq ..; bytes 2, 3: 32 further
+            const uint32_t lo = __byte_perm(w[0][v], w[1][v], half ? 0x7362 : 0x5140);   // the two keys' bytes, alternating
+            const uint32_t hi = __byte_perm(w[2][v], w[3][v], half ? 0x7362 : 0x5140);
             const int gr = (v * 64 + half * 32) / kGroup;
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-              mma_16n8<F16>(o[t][v * 4 + half * 2], a0, pb[t][gr][0], pb[t][gr][1]);
-              mma_16n8<F16>(o[t][v * 4 + half * 2 + 1], a1, pb[t][gr][0], pb[t][gr][1]);
+            for (int e = 0; e < 2; ++e) {
+              uint32_t a[4];
+              split_codes(__byte_perm(lo, 0x64646464u, e ? 0x4342 : 0x4140), a[0], a[1]);
+              split_codes(__byte_perm(hi, 0x64646464u, e ? 0x4342 : 0x4140), a[2], a[3]);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) mma_16n8_f16(o[t][v * 4 + half * 2 + e], a, pb[t][gr][0], pb[t][gr][1]);
             }
           }
       }
       __syncwarp();                                           // every lane has read the stage: it may be filled again
       feed();
+      ++done;
+      st = st + 1 == kKvStages ? 0 : st + 1;
+      phase ^= st == 0 ? 1 : 0;
     }
     if (!ok) break;
 
     // The part's rows: sums over the lanes of a row, then o or the workspace.  Rows 2 qd (+ 1), d = 64 v + 32 half + 4 gq + 0 .. 3.
     const int64_t slot_at = 2 * worker + (opening ? 0 : 1);
+    const float up = 1.f / vdown;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -619,76 +679,96 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
           for (int k = 0; k < NG; ++k) corr[t][i][k] += __shfl_xor_sync(0xffffffffu, corr[t][i][k], s);
         }
         if (r >= rows) continue;
-        const float inv = whole ? (m[t][i] == -INFINITY && l[t][i] == 0.f ? 0.f : 1.f / l[t][i]) : 1.f;
+        const bool none = room[t][i] == -INFINITY && l[t][i] == 0.f;   // no key was there (its pages were not): zeros
+        const float inv = !whole ? 1.f : none ? 0.f : 1.f / l[t][i];
         float *part = g.part_o + (slot_at * 16 + r) * D;
         uint16_t *out = g.b + slot * g.b_row + int64_t(head * g.per + row0 + r) * g.b_head;
 #pragma unroll
         for (int v = 0; v < kWordsV; ++v)
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            const int d = v * 64 + half * 32 + gq * 4;
+            const int d = v * 64 + half * 32 + gq * 4, k = v * 4 + half * 2;
             const float c = corr[t][i][(v * 64 + half * 32) / kGroup];
-            const float y0 = (o[t][v * 4 + half * 2][i] + c) * inv, y1 = (o[t][v * 4 + half * 2][i + 2] + c) * inv;
-            const float y2 = (o[t][v * 4 + half * 2 + 1][i] + c) * inv, y3 = (o[t][v * 4 + half * 2 + 1][i + 2] + c) * inv;
+            const float y0 = fmaf(o[t][k][i], up, c) * inv, y1 = fmaf(o[t][k][i + 2], up, c) * inv;
+            const float y2 = fmaf(o[t][k + 1][i], up, c) * inv, y3 = fmaf(o[t][k + 1][i + 2], up, c) * inv;
             if (whole) *reinterpret_cast<uint2 *>(out + d) = make_uint2(pack_16x2<F16>(y0, y1), pack_16x2<F16>(y2, y3));
             else *reinterpret_cast<float4 *>(part + d) = make_float4(y0, y1, y2, y3);
           }
-        if (!whole && gq == 0) {
-          g.part_ml[(slot_at * 16 + r) * 2] = m[t][i];
-          g.part_ml[(slot_at * 16 + r) * 2 + 1] = l[t][i];
-        }
+        if (!whole && gq == 0)
+          *reinterpret_cast<float2 *>(g.part_ml + (slot_at * 16 + r) * 2) = make_float2(room[t][i] == -INFINITY ? -INFINITY : m[t][i], l[t][i]);
       }
-    if (x < w_hi) use = seek(x);
+    use.tile = last;
+    if (last == use.tiles && done < count) next_item(use);
   }
   // After a wait that gave up, the copies in flight land (bounded) before the warp leaves its ring.
   if (!ok)
-    for (int64_t i = max(x, fx - kKvStages); i < fx; ++i)
-      sm100::mbar_wait(&full[int(i - w_lo) % kKvStages], uint32_t(int(i - w_lo) / kKvStages) & 1, wl);
+    for (int i = done; i < filled; ++i) {
+      sm100::mbar_wait(&full[st], phase, wl);
+      st = st + 1 == kKvStages ? 0 : st + 1;
+      phase ^= st == 0 ? 1 : 0;
+    }
 }
 
-// One CTA per (slot, item): merges the parts of an item that several workers hold, in key order; zeros for an empty slot.
-// Threads: D columns x 256 / D rows at a time.
+// Merges the parts of an item that several workers hold, in key order; zeros for an empty slot.  grid (slots x items, row
+// blocks), four warps: a warp takes 128 / D rows, D / 4 lanes of four columns each, and goes over the parts D / 4 at a time: lane j
+// fetches part j's (m, l) of the row, the maximum and the weights are shuffles, and the columns' loads of eight parts are in
+// flight together.  (A thread per column that walks the parts one by one costs two dependent loads a part: 116 us in the
+// place of 20 for 16 rows of 33 slots cut into 40 parts.)
 template <int D, bool F16>
-__global__ void __launch_bounds__(256) kv4_merge_kernel(const __grid_constant__ Kv4Args g) {
-  __shared__ int32_t sums[2][8];
+__global__ void __launch_bounds__(128) kv4_merge_kernel(const __grid_constant__ Kv4Args g) {
+  constexpr int kLanes = D / 4, kRows = 32 / kLanes;
   const int items = g.hkv * g.rb, slot = int(blockIdx.x) / items, item = int(blockIdx.x) % items;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, sub = lane / kLanes, col = lane % kLanes;
+  const int head = item / g.rb, row0 = (item % g.rb) * 16;
+  const int r = (int(blockIdx.y) * 4 + int(threadIdx.x >> 5)) * kRows + sub;
+  const bool live = r < min(16, g.per - row0);
   pdl_enter();
-  int total = 0, prior = 0;
-  for (int s = threadIdx.x; s < g.slots; s += 256) {
-    const int n = kv4_tiles(g, g.lens[s]);
-    total += n;
-    prior += s < slot ? n : 0;
-  }
-  total = __reduce_add_sync(0xffffffffu, total);
-  prior = __reduce_add_sync(0xffffffffu, prior);
-  if (lane == 0) sums[0][warp] = total, sums[1][warp] = prior;
-  __syncthreads();
-  total = prior = 0;
-  for (int w = 0; w < 8; ++w) total += sums[0][w], prior += sums[1][w];
-  const int tiles = kv4_tiles(g, g.lens[slot]);
-  const int head = item / g.rb, row0 = (item % g.rb) * 16, rows = min(16, g.per - row0);
-  const int d = threadIdx.x % D;
-  const int64_t all = int64_t(total) * items, n = min(int64_t(g.workers), all);
-  const int64_t t0 = int64_t(prior) * items + int64_t(item) * tiles;
-  int64_t w0 = 0, w1 = -1;
+  const int before = g.before[slot], tiles = g.before[slot + 1] - before;
+  const int64_t total = int64_t(g.before[g.slots]) * items, n = min(int64_t(g.workers), total);
+  const int64_t t0 = int64_t(before) * items + int64_t(item) * tiles;
+  int64_t w0 = 0;
+  int parts = 0, first = 0;                                    // first: the part of worker w0 is its last, not its opening one
   if (tiles > 0) {
-    w0 = kv4_worker(t0, all, n), w1 = kv4_worker(t0 + tiles - 1, all, n);
-    if (w0 == w1) return;                                      // one worker held the whole item and wrote it
+    w0 = kv4_worker(t0, total, n);
+    parts = int(kv4_worker(t0 + tiles - 1, total, n) - w0) + 1;
+    if (parts == 1) return;                                    // one worker held the whole item and wrote it
+    first = kv4_start(w0, total, n) < t0 ? 1 : 0;
   }
-  for (int r = threadIdx.x / D; r < rows; r += 256 / D) {
-    float top = -INFINITY, L = 0.f, O = 0.f;
-    auto at = [&](int64_t w) { return (2 * w + (kv4_start(w, all, n) >= t0 ? 0 : 1)) * 16 + r; };
-    for (int64_t w = w0; w <= w1; ++w) top = fmaxf(top, g.part_ml[at(w) * 2]);
-    for (int64_t w = w0; w <= w1; ++w) {
-      const float mw = g.part_ml[at(w) * 2];
-      const float e = mw == -INFINITY ? (g.part_ml[at(w) * 2 + 1] == 0.f ? 0.f : 1.f) : ex2_fast(mw - top);
-      L += g.part_ml[at(w) * 2 + 1] * e;
-      O += g.part_o[at(w) * D + d] * e;
+  float top = -INFINITY, L = 0.f;
+  float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int rr = live ? r : 0;
+  for (int j0 = 0; j0 < parts; j0 += kLanes) {
+    const int j = j0 + col;
+    float m = -INFINITY, l = 0.f;
+    if (j < parts) {
+      const float2 ml = *reinterpret_cast<const float2 *>(g.part_ml + ((2 * (w0 + j) + (j == 0 ? first : 0)) * 16 + rr) * 2);
+      m = ml.x, l = ml.y;
     }
-    const float y = top == -INFINITY && L == 0.f ? 0.f : O / L;
-    g.b[slot * g.b_row + int64_t(head * g.per + row0 + r) * g.b_head + d] = uint16_t(pack_16x2<F16>(y, y) & 0xffffu);
+    float now = m;
+#pragma unroll
+    for (int s = 1; s < kLanes; s *= 2) now = fmaxf(now, __shfl_xor_sync(0xffffffffu, now, s));
+    now = fmaxf(now, top);
+    const float back = now == top ? 1.f : ex2_fast(top - now);
+    float e = m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2_fast(m - now);   // l of a part without a maximum: 0, or NaN to pass on
+    float part = l * e;
+#pragma unroll
+    for (int s = 1; s < kLanes; s *= 2) part += __shfl_xor_sync(0xffffffffu, part, s);
+    L = L * back + part;
+    O.x *= back, O.y *= back, O.z *= back, O.w *= back;
+    top = now;
+    const int here = min(kLanes, parts - j0);
+#pragma unroll 8
+    for (int k = 0; k < here; ++k) {
+      const float w = __shfl_sync(0xffffffffu, e, k, kLanes);
+      const int64_t at = ((2 * (w0 + j0 + k) + (j0 + k == 0 ? first : 0)) * 16 + rr) * D + 4 * col;
+      const float4 o = *reinterpret_cast<const float4 *>(g.part_o + at);
+      O.x = fmaf(o.x, w, O.x), O.y = fmaf(o.y, w, O.y), O.z = fmaf(o.z, w, O.z), O.w = fmaf(o.w, w, O.w);
+    }
   }
+  if (!live) return;
+  const float inv = top == -INFINITY && L == 0.f ? 0.f : 1.f / L;
+  *reinterpret_cast<uint2 *>(g.b + slot * g.b_row + int64_t(head * g.per + row0 + r) * g.b_head + 4 * col) =
+      make_uint2(pack_16x2<F16>(O.x * inv, O.y * inv), pack_16x2<F16>(O.z * inv, O.w * inv));
 }
 
 // Workers of a launch: one warp each, as many as are resident at once.
@@ -698,7 +778,7 @@ static int kv4_workers(const ptsim_kv4_params &p, int sm_count) {
 
 int64_t kv4_workspace(const ptsim_desc &d, int sm_count) {
   const ptsim_kv4_params &p = d.p.kv4;
-  return 2 * int64_t(kv4_workers(p, sm_count)) * 16 * (p.dim + 2) * int64_t(sizeof(float));
+  return (2 * int64_t(kv4_workers(p, sm_count)) * 16 * (p.dim + 2) + p.slots + 1) * int64_t(sizeof(float));
 }
 
 template <int D, int NG, int NT, bool F16>
@@ -707,7 +787,9 @@ static int run_kv4_attn(const Kv4Args &g, const LaunchCtx &c) {
   constexpr int fixed = kKvWarps * kKvStages * (kKvTile * (D + 8 * NG) + 12) + 16;
   PTSIM_CUDA((smem_limit_once<kern>(fixed + 4 * (PTSIM_KV4_SLOTS + 1), c.device)));
   PTSIM_CUDA(launch_pdl(kern, dim3(unsigned(g.workers / kKvWarps)), dim3(kKvWarps * 32), fixed + 4 * (g.slots + 1), c.stream, g));
-  PTSIM_CUDA(launch_pdl(kv4_merge_kernel<D, F16>, dim3(unsigned(g.slots * g.hkv * g.rb)), dim3(256), 0, c.stream, g));
+  const int rows = g.per < 16 ? g.per : 16;
+  PTSIM_CUDA(launch_pdl(kv4_merge_kernel<D, F16>, dim3(unsigned(g.slots * g.hkv * g.rb), unsigned(ceil_div(rows * D, 512))), dim3(128), 0,
+                        c.stream, g));
   return PTSIM_OK;
 }
 
@@ -747,6 +829,7 @@ int launch_kv4(const ptsim_desc &d, void *const *ptrs, void *ws, size_t ws_bytes
   g.hkv = int(p.hkv);
   g.pages = int(p.pages);
   g.page_size = int(p.page_size);
+  g.page_log = p.page_size == 16 ? 4 : p.page_size == 32 ? 5 : p.page_size == 64 ? 6 : 7;
   g.max_pages = int(p.max_pages);
   g.stall = (d.flags & PTSIM_FLAG_TEST_STALL) ? 1 : 0;
   if (attn) {
@@ -760,6 +843,7 @@ int launch_kv4(const ptsim_desc &d, void *const *ptrs, void *ws, size_t ws_bytes
     if (reinterpret_cast<uintptr_t>(ws) % 16 != 0) return fail(PTSIM_E_ARGS, "workspace is not 16-byte aligned");
     g.part_o = static_cast<float *>(ws);
     g.part_ml = g.part_o + 2 * int64_t(g.workers) * 16 * p.dim;
+    g.before = reinterpret_cast<int32_t *>(g.part_ml + 2 * int64_t(g.workers) * 16 * 2);
   }
   const bool f16 = d.arg_dtype[p.a_arg] == PTSIM_DT_F16;
   switch (p.dim / p.group + (p.dim == 128 ? 10 : 0) + (f16 ? 100 : 0)) {
