@@ -315,7 +315,7 @@ typedef struct ptsim_itab_params {
  * sequence keep their values.  Element (token t, head h, d) of x lies at x_off + t x_row + h x_head + d of argument
  * x_arg (q, k, v may be parts of one argument); offsets and strides are multiples of 8 elements.  A table that
  * descends or leaves the tokens records PTSIM_E_OOB and its sequence is skipped.  bf16 or fp16 throughout; dim 64 or
- * 128; scale > 0, scores scale q.k below 2^30; at most PTSIM_PACKED_SEQS sequences.  One partition unit. */
+ * 128; scale > 0, scores scale q.k below 2^20; at most PTSIM_PACKED_SEQS sequences.  One partition unit. */
 #define PTSIM_PACKED_SEQS 4096
 typedef struct ptsim_pattn_params {
   int64_t q_tokens, k_tokens, seqs, hq, hkv, dim;
@@ -340,7 +340,7 @@ typedef struct ptsim_pattn_params {
  * tokens of slot s into rows of a and b, scale * code + minimum in fp32 rounded to their type; rows of no slot are
  * left alone.  ATTN_KV4: a = q, b = o,
  * rows of one token per slot: query head h of slot s attends over the lens[s] cached tokens of KV head h / (hq / hkv); a
- * slot of length 0 gives zeros.  Element (row t, head h, d) of x lies at x_off + t x_row + h x_head + d, offsets and
+ * slot of length 0 gives zeros (scale > 0, scores below 2^20).  Element (row t, head h, d) of x lies at x_off + t x_row + h x_head + d, offsets and
  * strides multiples of 8 elements.  A token outside the table's row, or a page outside the pool, records PTSIM_E_OOB
  * and is not written, reads as zeros, is not attended to.  One partition unit. */
 #define PTSIM_KV4_PAGE_BYTES(hkv, page_size, dim, group) ((hkv) * (page_size) * ((dim) + 8 * ((dim) / (group))))

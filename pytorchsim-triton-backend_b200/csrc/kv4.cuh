@@ -20,7 +20,7 @@
 // without bank conflicts give words whose nibbles are the fragments.
 //
 // Bound: HBM, (D + 8 D / group) bytes per key and KV head (144 at D 128, group 64: 3.5 times fewer than bf16), and before
-// it the issue slots of the unpacking.  Work is one list of 32-key tiles over (slot, KV head), cut into equal contiguous
+// it the issue slots of the unpacking.  Work is one list of 64-key tiles over (slot, KV head), cut into equal contiguous
 // ranges, one per warp: a warp streams its tiles by bulk copies through a ring of its own (no barrier between warps) and keeps
 // the online softmax in registers.  Lengths are read on the device, so any raggedness is balanced to a tile.  A range that
 // holds only part of an item leaves (m, l, O) in the workspace and a second kernel (a programmatic dependent) merges the parts
@@ -32,8 +32,9 @@
 
 namespace ptsim {
 
-constexpr int kKvTile = 32;          // keys of a tile
-constexpr int kKvStages = 3;
+constexpr int kKvTile = 64;          // keys of a tile: what a warp is given and copies at once
+constexpr int kKvPass = 32;          // keys of one pass over the softmax
+constexpr int kKvStages = 2;
 constexpr int kKvWarps = 4;
 
 struct Kv4Args {
@@ -238,11 +239,24 @@ __device__ __forceinline__ void mma_16n8_f16(float (&d)[4], const uint32_t (&a)[
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same product onto c0 in the even columns and c1 in the odd ones.
+__device__ __forceinline__ void mma_16n8_first(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, float c0, float c1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+}
+
 // x = a pair of fp16 1024 + lo + 16 hi (codes lo, hi of a byte): the pairs lo - 8 and hi - 8, exact.
 __device__ __forceinline__ void split_codes(uint32_t x, uint32_t &lo, uint32_t &hi) {
   const uint32_t y = (x & 0xfff0fff0u) | 0x00080008u;                                    // 1032 + 16 hi
   asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(y));
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(hi) : "r"(y), "r"(0x2c002c00u), "r"(0xd488d488u));   // y / 16 - 72.5
+}
+
+// The pairs lo - 8 and 1032 + 16 hi.
+__device__ __forceinline__ void split_offset(uint32_t x, uint32_t &lo, uint32_t &hi) {
+  hi = (x & 0xfff0fff0u) | 0x00080008u;
+  asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(hi));
 }
 
 // How far (log2) a score may pass its row's reference before the reference moves.  The weight times the V scale is an fp16
@@ -274,7 +288,7 @@ __device__ __forceinline__ int64_t kv4_worker(int64_t tile, int64_t total, int64
 
 template <int D, int NG, int NT, bool F16>
 __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kernel(const __grid_constant__ Kv4Args g) {
-  constexpr int kStage = kKvTile * (D + 8 * NG);            // bytes of a tile: one block of 32 keys or two of 16
+  constexpr int kStage = kKvTile * (D + 8 * NG);            // bytes of a tile: two blocks of 32 keys or four of 16
   constexpr int kWordsK = D / 32, kWordsV = D / 64;         // words a lane takes of a K and of a V row
   constexpr int kGroup = D / NG;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -356,11 +370,11 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
   };
 
   // Producer side: lane k < parts holds the pool page of the k-th part of the tile that is copied next.
-  const int bs_log = min(g.page_log, 5), bs = 1 << bs_log, parts = kKvTile >> bs_log;
-  const uint32_t part_bytes = uint32_t(bs * (D + 8 * NG));
+  const int bs = 1 << min(g.page_log, 5), part_log = min(g.page_log, 6), parts = kKvTile >> part_log;   // a block's keys; a copy's
+  const uint32_t part_bytes = uint32_t((D + 8 * NG) << part_log);
   auto next_page = [&](const Cursor &c) {
     int page = -2;                                          // -2: no key of the slot lies there
-    const int first = c.tile * kKvTile + lane * bs;
+    const int first = c.tile * kKvTile + (lane << part_log);
     if (lane < parts && first < c.len) {
       page = g.table[int64_t(c.slot) * g.max_pages + (first >> g.page_log)];
       if (page < 0 || page >= g.pages) page = -1;
@@ -377,8 +391,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
     }
     __syncwarp();
     if (page >= 0 && !withheld) {
-      const int block = ((c.tile * kKvTile + lane * bs) & ((1 << g.page_log) - 1)) >> bs_log;
-      const uint8_t *src = g.pool + (int64_t(page) * g.hkv + c.head) * g.record + uint32_t(block) * part_bytes;
+      const int part = ((c.tile * kKvTile + (lane << part_log)) & ((1 << g.page_log) - 1)) >> part_log;
+      const uint8_t *src = g.pool + (int64_t(page) * g.hkv + c.head) * g.record + uint32_t(part) * part_bytes;
       sm100::bulk_load_g2s(ring + fill_st * kStage + lane * part_bytes, src, part_bytes, &full[fill_st]);
     }
     fill_st = fill_st + 1 == kKvStages ? 0 : fill_st + 1;
@@ -413,7 +427,9 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
     const bool whole = first == 0 && last == use.tiles, opening = done == 0;
 
     uint32_t qb[NT][kWordsK][4];                            // fp16 pairs of d = 32 b + 8 qd + 0 .. 7 of row gq
-    float qsum[NT][2][NG], sl[NT][2];                       // of rows 2 qd and 2 qd + 1: sums per group, scale
+    // Of rows 2 qd and 2 qd + 1: sums per group, what the operands' offsets add to a score (the odd pairs of K are
+    // 1032 + 16 c, and their q is divided by 16: 72.5 more than c - 8), scale.
+    float qsum[NT][2][NG], qoff[NT][2][NG], sl[NT][2];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       const int r = t * 8 + gq;
@@ -444,21 +460,36 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
 #pragma unroll
           for (int i = 0; i < 4; ++i) qb[t][b][i] = pack_16x2<true>(lo_bf16(qb[t][b][i]) * down, hi_bf16(qb[t][b][i]) * down);
       }
+      float odd[NG];
 #pragma unroll
-      for (int b = 0; b < kWordsK; ++b)
+      for (int i = 0; i < NG; ++i) odd[i] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s[b * 32 / kGroup] += lo_f32<true>(qb[t][b][i]) + hi_f32<true>(qb[t][b][i]);
+      for (int b = 0; b < kWordsK; ++b) {
+        s[b * 32 / kGroup] += lo_f32<true>(qb[t][b][0]) + hi_f32<true>(qb[t][b][0]) + lo_f32<true>(qb[t][b][2]) + hi_f32<true>(qb[t][b][2]);
+#pragma unroll
+        for (int i = 1; i < 4; i += 2) {                    // the sixteenth is what the products see, its rounding included
+          const float x0 = lo_f32<true>(qb[t][b][i]) * 0.0625f, x1 = hi_f32<true>(qb[t][b][i]) * 0.0625f;
+          qb[t][b][i] = pack_16x2<true>(x0, x1);
+          odd[b * 32 / kGroup] += lo_f32<true>(qb[t][b][i]) + hi_f32<true>(qb[t][b][i]);
+        }
+      }
 #pragma unroll
       for (int i = 0; i < NG; ++i) {
+        odd[i] += __shfl_xor_sync(0xffffffffu, odd[i], 1);
+        odd[i] += __shfl_xor_sync(0xffffffffu, odd[i], 2);
         s[i] += __shfl_xor_sync(0xffffffffu, s[i], 1);
         s[i] += __shfl_xor_sync(0xffffffffu, s[i], 2);
-        qsum[t][0][i] = __shfl_sync(0xffffffffu, s[i], 8 * qd);
-        qsum[t][1][i] = __shfl_sync(0xffffffffu, s[i], 8 * qd + 4);
+        s[i] = fmaf(16.f, odd[i], s[i]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          qsum[t][k][i] = __shfl_sync(0xffffffffu, s[i], 8 * qd + 4 * k);
+          qoff[t][k][i] = -1160.f * __shfl_sync(0xffffffffu, odd[i], 8 * qd + 4 * k);
+        }
       }
       sl[t][0] = __shfl_sync(0xffffffffu, back, 8 * qd);
       sl[t][1] = __shfl_sync(0xffffffffu, back, 8 * qd + 4);
     }
-    // m: the rows' references (log2), 0 until a score has been seen (seen < 0: none); room: the score that moves it.
+    // m: the rows' references (log2), 0 before the first score; room: the unscaled score that moves it, -inf before the first.
     float m[NT][2], room[NT][2], l[NT][2], corr[NT][2][NG], o[NT][D / 16][4];
     float vdown = 1.f;                                      // power of two on the V scales (bf16 caches)
     uint32_t vroom = 0;                                     // largest V scale (bits) it allows
@@ -480,10 +511,14 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
         ok = false;
         break;
       }
-      const uint8_t *buf = ring + st * kStage;
+      const int there = good[st];
+#pragma unroll 1
+      for (int pass = 0; pass < kKvTile / kKvPass; ++pass) {
+      const uint8_t *buf = ring + st * kStage + pass * (kKvPass * (D + 8 * NG));
       // Keys past the length, or whose page is not there, take no part: score -inf and parameters 0.
-      const int left = len - tile * kKvTile, there = good[st];
-      const bool partial = left < kKvTile || there != (1 << parts) - 1;
+      const int left = len - tile * kKvTile - pass * kKvPass;
+      if (left <= 0) break;
+      const bool partial = left < kKvPass || there != (1 << parts) - 1;
       float z[2][NT][4];                                    // [step][row block][key gq: rows 2 qd, + 1; key gq + 8: the same]
       uint32_t vp[2][2][NG];
 #pragma unroll
@@ -507,18 +542,18 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
         }
         float acc[NT][NG][4];
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
-#pragma unroll
-          for (int i = 0; i < NG; ++i) acc[t][i][0] = acc[t][i][1] = acc[t][i][2] = acc[t][i][3] = 0.f;
-#pragma unroll
         for (int b = 0; b < kWordsK; ++b)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {                     // bytes 0 and 2: d = 0, 1 | 2, 3; bytes 1 and 3: 4, 5 | 6, 7
             uint32_t a[4];
-            split_codes(__byte_perm(wa[b], 0x64646464u, e ? 0x4341 : 0x4240), a[0], a[2]);
-            split_codes(__byte_perm(wb[b], 0x64646464u, e ? 0x4341 : 0x4240), a[1], a[3]);
+            split_offset(__byte_perm(wa[b], 0x64646464u, e ? 0x4341 : 0x4240), a[0], a[2]);
+            split_offset(__byte_perm(wb[b], 0x64646464u, e ? 0x4341 : 0x4240), a[1], a[3]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_16n8_f16(acc[t][b * 32 / kGroup], a, qb[t][b][2 * e], qb[t][b][2 * e + 1]);
+            for (int t = 0; t < NT; ++t) {
+              if (e == 0 && b * 32 % kGroup == 0) mma_16n8_first(acc[t][b * 32 / kGroup], a, qb[t][b][0], qb[t][b][1], qoff[t][0][b * 32 / kGroup],
+                                                                          qoff[t][1][b * 32 / kGroup]);
+              else mma_16n8_f16(acc[t][b * 32 / kGroup], a, qb[t][b][2 * e], qb[t][b][2 * e + 1]);
+            }
           }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
@@ -534,14 +569,14 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
               for (int n = 1; n < NG; ++n) s = fmaf(mid[n], qsum[t][i][n], s);
 #pragma unroll
               for (int n = 0; n < NG; ++n) s = fmaf(a[n], acc[t][n][2 * k + i], s);
-              z[h][t][2 * k + i] = s * sl[t][i];
+              z[h][t][2 * k + i] = s;
             }
         }
         if (partial) {
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const int key = h * 16 + k * 8 + gq;
-            if (key < left && ((there >> (small ? h : 0)) & 1)) continue;
+            if (key < left && ((there >> ((pass * kKvPass + h * 16) >> part_log)) & 1)) continue;
 #pragma unroll
             for (int t = 0; t < NT; ++t) z[h][t][2 * k] = z[h][t][2 * k + 1] = -INFINITY;
 #pragma unroll
@@ -593,11 +628,12 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
             float top = fmaxf(fmaxf(z[0][t][i], z[0][t][i + 2]), fmaxf(z[1][t][i], z[1][t][i + 2]));
 #pragma unroll
             for (int s = 4; s < 32; s *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+            const float to = top * sl[t][i];
             float alpha = 1.f;
-            if (top > room[t][i] - kKvGrow<F16>) {          // past the reference, or the first score: nothing to rescale then
-              if (room[t][i] != -INFINITY) alpha = ex2_fast(m[t][i] - top);
-              m[t][i] = top;
-              room[t][i] = top + kKvGrow<F16>;
+            if (top > room[t][i] || (room[t][i] != -INFINITY && to > m[t][i])) {
+              if (room[t][i] != -INFINITY) alpha = ex2_fast(m[t][i] - to);    // the first score: nothing to rescale
+              m[t][i] = to;
+              room[t][i] = top + kKvGrow<F16> / sl[t][i];
             }
             l[t][i] *= alpha;
 #pragma unroll
@@ -621,7 +657,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
           }
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            const float p0 = ex2_fast(z[h][t][2 * k] - m[t][0]), p1 = ex2_fast(z[h][t][2 * k + 1] - m[t][1]);
+            const float p0 = ex2_fast(fmaf(z[h][t][2 * k], sl[t][0], -m[t][0]));
+            const float p1 = ex2_fast(fmaf(z[h][t][2 * k + 1], sl[t][1], -m[t][1]));
             l[t][0] += p0;
             l[t][1] += p1;
 #pragma unroll
@@ -655,6 +692,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
               for (int t = 0; t < NT; ++t) mma_16n8_f16(o[t][v * 4 + half * 2 + e], a, pb[t][gr][0], pb[t][gr][1]);
             }
           }
+      }
       }
       __syncwarp();                                           // every lane has read the stage: it may be filled again
       feed();
