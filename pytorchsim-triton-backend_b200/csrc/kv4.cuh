@@ -246,16 +246,22 @@ __device__ __forceinline__ void mma_16n8_first(float (&d)[4], const uint32_t (&a
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+
 // x = a pair of fp16 1024 + lo + 16 hi (codes lo, hi of a byte): the pairs lo - 8 and hi - 8, exact.
 __device__ __forceinline__ void split_codes(uint32_t x, uint32_t &lo, uint32_t &hi) {
-  const uint32_t y = (x & 0xfff0fff0u) | 0x00080008u;                                    // 1032 + 16 hi
+  const uint32_t y = and_or(x, 0xfff0fff0u, 0x00080008u);                                // 1032 + 16 hi
   asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(y));
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(hi) : "r"(y), "r"(0x2c002c00u), "r"(0xd488d488u));   // y / 16 - 72.5
 }
 
 // The pairs lo - 8 and 1032 + 16 hi.
 __device__ __forceinline__ void split_offset(uint32_t x, uint32_t &lo, uint32_t &hi) {
-  hi = (x & 0xfff0fff0u) | 0x00080008u;
+  hi = and_or(x, 0xfff0fff0u, 0x00080008u);
   asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(hi));
 }
 
