@@ -495,15 +495,15 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
       sl[t][0] = __shfl_sync(0xffffffffu, back, 8 * qd);
       sl[t][1] = __shfl_sync(0xffffffffu, back, 8 * qd + 4);
     }
-    // m: the rows' references (log2), 0 before the first score; room: the unscaled score that moves it, -inf before the first.
-    float m[NT][2], room[NT][2], l[NT][2], corr[NT][2][NG], o[NT][D / 16][4];
+    // nm: the rows' references (log2), negated, 0 before the first score; room: the unscaled score that moves it, -inf before the first.
+    float nm[NT][2], room[NT][2], l[NT][2], corr[NT][2][NG], o[NT][D / 16][4];
     float vdown = 1.f;                                      // power of two on the V scales (bf16 caches)
     uint32_t vroom = 0;                                     // largest V scale (bits) it allows
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        m[t][i] = l[t][i] = 0.f;
+        nm[t][i] = l[t][i] = 0.f;
         room[t][i] = -INFINITY;
 #pragma unroll
         for (int k = 0; k < NG; ++k) corr[t][i][k] = 0.f;
@@ -567,16 +567,14 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
 #pragma unroll
           for (int i = 0; i < NG; ++i) a[i] = lo_f32<F16>(kp[k][i]), mid[i] = fmaf(8.f, a[i], hi_f32<F16>(kp[k][i]));
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
+          for (int t = 0; t < NT; ++t) {
+            float2 s2 = __fmul2_rn(make_float2(mid[0], mid[0]), make_float2(qsum[t][0][0], qsum[t][1][0]));
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float s = mid[0] * qsum[t][i][0];
+            for (int n = 1; n < NG; ++n) s2 = __ffma2_rn(make_float2(mid[n], mid[n]), make_float2(qsum[t][0][n], qsum[t][1][n]), s2);
 #pragma unroll
-              for (int n = 1; n < NG; ++n) s = fmaf(mid[n], qsum[t][i][n], s);
-#pragma unroll
-              for (int n = 0; n < NG; ++n) s = fmaf(a[n], acc[t][n][2 * k + i], s);
-              z[h][t][2 * k + i] = s;
-            }
+            for (int n = 0; n < NG; ++n) s2 = __ffma2_rn(make_float2(a[n], a[n]), make_float2(acc[t][n][2 * k], acc[t][n][2 * k + 1]), s2);
+            z[h][t][2 * k] = s2.x, z[h][t][2 * k + 1] = s2.y;
+          }
         }
         if (partial) {
 #pragma unroll
@@ -636,9 +634,9 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
             for (int s = 4; s < 32; s *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
             const float to = top * sl[t][i];
             float alpha = 1.f;
-            if (top > room[t][i] || (room[t][i] != -INFINITY && to > m[t][i])) {
-              if (room[t][i] != -INFINITY) alpha = ex2_fast(m[t][i] - to);    // the first score: nothing to rescale
-              m[t][i] = to;
+            if (top > room[t][i] || (room[t][i] != -INFINITY && to > -nm[t][i])) {
+              if (room[t][i] != -INFINITY) alpha = ex2_fast(-nm[t][i] - to);    // the first score: nothing to rescale
+              nm[t][i] = -to;
               room[t][i] = top + kKvGrow<F16> / sl[t][i];
             }
             l[t][i] *= alpha;
@@ -663,15 +661,17 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
           }
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
-            const float p0 = ex2_fast(fmaf(z[h][t][2 * k], sl[t][0], -m[t][0]));
-            const float p1 = ex2_fast(fmaf(z[h][t][2 * k + 1], sl[t][1], -m[t][1]));
-            l[t][0] += p0;
-            l[t][1] += p1;
+            float2 p = __ffma2_rn(make_float2(z[h][t][2 * k], z[h][t][2 * k + 1]), make_float2(sl[t][0], sl[t][1]),
+                                  make_float2(nm[t][0], nm[t][1]));
+            p.x = ex2_fast(p.x), p.y = ex2_fast(p.y);
+            const float2 sum = __fadd2_rn(make_float2(l[t][0], l[t][1]), p);
+            l[t][0] = sum.x, l[t][1] = sum.y;
 #pragma unroll
             for (int i = 0; i < NG; ++i) {
-              corr[t][0][i] = fmaf(p0, mid[i], corr[t][0][i]);
-              corr[t][1][i] = fmaf(p1, mid[i], corr[t][1][i]);
-              pb[t][i][k] = transpose_8x8(pack_16x2<true>(p0 * a[i], p1 * a[i]));
+              const float2 c = __ffma2_rn(p, make_float2(mid[i], mid[i]), make_float2(corr[t][0][i], corr[t][1][i]));
+              corr[t][0][i] = c.x, corr[t][1][i] = c.y;
+              const float2 w = __fmul2_rn(p, make_float2(a[i], a[i]));
+              pb[t][i][k] = transpose_8x8(pack_16x2<true>(w.x, w.y));
             }
           }
         }
@@ -739,7 +739,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
             else *reinterpret_cast<float4 *>(part + d) = make_float4(y0, y1, y2, y3);
           }
         if (!whole && gq == 0)
-          *reinterpret_cast<float2 *>(g.part_ml + (slot_at * 16 + r) * 2) = make_float2(room[t][i] == -INFINITY ? -INFINITY : m[t][i], l[t][i]);
+          *reinterpret_cast<float2 *>(g.part_ml + (slot_at * 16 + r) * 2) = make_float2(room[t][i] == -INFINITY ? -INFINITY : -nm[t][i], l[t][i]);
       }
     use.tile = last;
     if (last == use.tiles && done < count) next_item(use);
