@@ -47,7 +47,7 @@ struct Kv4Args {
   int32_t pages, page_size, page_log, max_pages;
   float sl;                          // scale * log2 e
   float *part_o, *part_ml;           // [2 * workers][16][D] and [2 * workers][16][2]
-  int32_t *before;                   // [slots + 1] tiles before a slot, for the merge
+  int32_t *before;                   // [slots + 1] units of an item before a slot (kv4_units), for the merge
   int32_t workers, stall;
 };
 
@@ -287,10 +287,15 @@ __device__ __forceinline__ int kv4_tiles(const Kv4Args &g, int len) {
   return (len + kKvTile - 1) / kKvTile;
 }
 
-// Work list: tiles before slot s times the items (KV head, row block) of a slot; worker w takes tiles [w total / n,
-// (w + 1) total / n).
-__device__ __forceinline__ int64_t kv4_start(int64_t w, int64_t total, int64_t n) { return w * total / n; }
-__device__ __forceinline__ int64_t kv4_worker(int64_t tile, int64_t total, int64_t n) { return ((tile + 1) * n - 1) / total; }
+// Work list: every item (KV head, row block) of every slot that holds keys, kKvItemCost units and then a unit per tile; worker w
+// takes units [w c, (w + 1) c), c = kv4_share.  The cost stands for what a part costs beside its tiles (q fetched and
+// converted, sums over lanes, the part written: about one tile); without it the workers that got many short items ended a
+// fifth after the others (64 slots of up to 8191 keys).
+constexpr int kKvItemCost = 1;
+__device__ __forceinline__ int kv4_units(int tiles) { return tiles > 0 ? tiles + kKvItemCost : 0; }
+// Units of a worker: the list's length over the workers, rounded up (the last workers may get none, the longest range is
+// no longer than in an even cut).
+__device__ __forceinline__ uint32_t kv4_share(uint32_t total, int workers) { return (total + uint32_t(workers) - 1) / uint32_t(workers); }
 
 template <int D, int NG, int NT, bool F16>
 __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kernel(const __grid_constant__ Kv4Args g) {
@@ -301,8 +306,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
   uint8_t *ring = smem + (threadIdx.x >> 5) * kKvStages * kStage;
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + kKvWarps * kKvStages * kStage) + (threadIdx.x >> 5) * kKvStages;
   int32_t *good = reinterpret_cast<int32_t *>(smem + kKvWarps * kKvStages * (kStage + 8)) + (threadIdx.x >> 5) * kKvStages;
-  int32_t *before = reinterpret_cast<int32_t *>(smem + kKvWarps * kKvStages * (kStage + 12));   // [slots + 1] tiles before a slot
-  __shared__ int32_t sums[kKvWarps];
+  int32_t *before = reinterpret_cast<int32_t *>(smem + kKvWarps * kKvStages * (kStage + 12));   // [slots + 1] units of an item before a slot
+  __shared__ int32_t sums[2 * kKvWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, qd = lane & 3;
   const uint32_t wl = g.stall ? kTestWaitUs : kWaitUs;
   if (lane == 0) {
@@ -311,55 +316,65 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
   }
   pdl_enter();
 
-  // before[s]: a thread sums a run of slots, the runs are scanned over the CTA.
+  // before[s], and how many slots before s hold keys: a thread sums a run of slots, the runs are scanned over the CTA.
+  uint16_t *held = reinterpret_cast<uint16_t *>(before + g.slots + 1);
   const int run = (g.slots + kKvWarps * 32 - 1) / (kKvWarps * 32), s_lo = threadIdx.x * run;
-  int mine = 0;
-  for (int s = s_lo; s < min(s_lo + run, g.slots); ++s) mine += kv4_tiles(g, g.lens[s]);
-  int scan = mine;
+  int mine = 0, some = 0;
+  for (int s = s_lo; s < min(s_lo + run, g.slots); ++s) {
+    const int u = kv4_units(kv4_tiles(g, g.lens[s]));
+    mine += u;
+    some += u > 0;
+  }
+  int scan = mine, scan2 = some;
 #pragma unroll
   for (int o = 1; o < 32; o *= 2) {
-    const int up = __shfl_up_sync(0xffffffffu, scan, o);
-    if (lane >= o) scan += up;
+    const int up = __shfl_up_sync(0xffffffffu, scan, o), up2 = __shfl_up_sync(0xffffffffu, scan2, o);
+    if (lane >= o) scan += up, scan2 += up2;
   }
-  if (lane == 31) sums[warp] = scan;
+  if (lane == 31) sums[warp] = scan, sums[kKvWarps + warp] = scan2;
   __syncthreads();
-  for (int w = 0; w < warp; ++w) scan += sums[w];
-  int at = scan - mine;
+  for (int w = 0; w < warp; ++w) scan += sums[w], scan2 += sums[kKvWarps + w];
+  int at = scan - mine, at2 = scan2 - some;
   for (int s = s_lo; s < min(s_lo + run, g.slots); ++s) {
     before[s] = at;
-    at += kv4_tiles(g, g.lens[s]);
+    held[s] = uint16_t(at2);
+    const int u = kv4_units(kv4_tiles(g, g.lens[s]));
+    at += u;
+    at2 += u > 0;
   }
-  if (threadIdx.x == kKvWarps * 32 - 1) before[g.slots] = scan;
+  if (threadIdx.x == kKvWarps * 32 - 1) before[g.slots] = scan, held[g.slots] = uint16_t(scan2);
   __syncthreads();
   if (blockIdx.x == 0)
     for (int s = threadIdx.x; s <= g.slots; s += kKvWarps * 32) g.before[s] = before[s];
 
   const int items = g.hkv * g.rb;                           // items of a slot
-  const int64_t total = int64_t(before[g.slots]) * items;
-  const int64_t worker = int64_t(warp) * gridDim.x + blockIdx.x;
-  const int64_t n = min(int64_t(g.workers), total);
-  if (worker >= n) return;
-  const int64_t w_lo = kv4_start(worker, total, n), w_hi = kv4_start(worker + 1, total, n);
+  const uint32_t total = uint32_t(before[g.slots]) * uint32_t(items), share = kv4_share(total, g.workers);
+  const uint32_t worker = uint32_t(warp) * gridDim.x + blockIdx.x;
+  const uint64_t from = uint64_t(worker) * share;
+  if (from >= total) return;
+  const uint32_t w_lo = uint32_t(from), w_hi = uint32_t(min(from + share, uint64_t(total)));
 
   // Position in the list: slot, its length and tiles, KV head and row block, tile of the item.
   struct Cursor {
     int slot, len, tiles, head, block, tile;
   };
-  auto seek = [&](int64_t x) {
+  // The tile that unit x belongs to (an item's first one for the units of its cost); *index: tiles before it in the list.
+  auto seek = [&](uint32_t x, uint32_t *index) {
     int lo = 0, hi = g.slots;                               // the last slot with before * items <= x
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
-      if (int64_t(before[mid]) * items <= x) lo = mid;
+      if (uint32_t(before[mid]) * uint32_t(items) <= x) lo = mid;
       else hi = mid;
     }
     Cursor c;
     c.slot = lo;
-    c.len = g.lens[lo];
-    c.tiles = before[lo + 1] - before[lo];
-    const uint32_t in = uint32_t(x - int64_t(before[lo]) * items), item = in / uint32_t(c.tiles);
-    c.head = int(item) / g.rb;
-    c.block = int(item) % g.rb;
-    c.tile = int(in % uint32_t(c.tiles));
+    const uint32_t units = uint32_t(before[lo + 1] - before[lo]), in = x - uint32_t(before[lo]) * uint32_t(items), item = in / units;
+    c.tiles = int(units) - kKvItemCost;
+    c.head = int(item);
+    c.block = 0;
+    if (g.rb > 1) c.head = int(item) / g.rb, c.block = int(item) % g.rb;
+    c.tile = max(0, int(in - item * units) - kKvItemCost);
+    *index = uint32_t(before[lo] - kKvItemCost * held[lo]) * uint32_t(items) + item * uint32_t(c.tiles) + uint32_t(c.tile);
     return c;
   };
   auto next_item = [&](Cursor &c) {
@@ -370,8 +385,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
     c.head = 0;
     do {
       ++c.slot;
-      c.tiles = c.slot < g.slots ? before[c.slot + 1] - before[c.slot] : 1;
-    } while (c.tiles == 0);
+      c.tiles = c.slot < g.slots ? before[c.slot + 1] - before[c.slot] - kKvItemCost : 1;
+    } while (c.tiles <= 0);
     c.len = c.slot < g.slots ? g.lens[c.slot] : 0;
   };
 
@@ -404,12 +419,17 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
     fill_st = fill_st + 1 == kKvStages ? 0 : fill_st + 1;
   };
 
-  Cursor use = seek(w_lo), fill = use;
-  const int count = int(w_hi - w_lo);
+  uint32_t index, end = uint32_t(before[g.slots] - kKvItemCost * held[g.slots]) * uint32_t(items);
+  Cursor use = seek(w_lo, &index);
+  use.len = g.lens[use.slot];
+  Cursor fill = use;
   int filled = 0, page = next_page(fill);
+  if (w_hi < total) seek(w_hi, &end);
+  const int count = int(end - index);                       // 0: units of an item's cost only
+  if (count == 0) return;
   auto feed = [&]() {                                       // copy the next tile, then fetch the pages of the one after it
     if (filled >= count) return;
-    copy(fill, page, g.stall && blockIdx.x == 0 && warp == 0 && filled == 0);   // test hook: armed, no copy in flight
+    copy(fill, page, g.stall && index == 0 && filled == 0);   // test hook: armed, no copy in flight
     if (++filled < count) {
       if (++fill.tile == fill.tiles) next_item(fill);
       page = next_page(fill);
@@ -709,7 +729,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
     if (!ok) break;
 
     // The part's rows: sums over the lanes of a row, then o or the workspace.  Rows 2 qd (+ 1), d = 64 v + 32 half + 4 gq + 0 .. 3.
-    const int64_t slot_at = 2 * worker + (opening ? 0 : 1);
+    const int64_t slot_at = 2 * int64_t(worker) + (opening ? 0 : 1);
     const float up = 1.f / vdown;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -754,9 +774,9 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
 }
 
 // Merges the parts of an item that several workers hold, in key order; zeros for an empty slot.  grid (slots x items, row
-// blocks), four warps: a warp takes 128 / D rows, D / 4 lanes of four columns each, and goes over the parts D / 4 at a time: lane j
-// fetches part j's (m, l) of the row, the maximum and the weights are shuffles, and the columns' loads of eight parts are in
-// flight together.  (A thread per column that walks the parts one by one costs two dependent loads a part: 116 us in the
+// blocks of 128 / D rows), D / 4 lanes of four columns a row.  Each of the four warps goes over a quarter of the parts, D / 4 at a
+// time: lane j fetches part j's (m, l) of the row, the maximum and the weights are shuffles, and the columns' loads of eight
+// parts are in flight together; the quarters meet in shared memory.  (A thread per column that walks the parts one by one costs two dependent loads a part: 116 us in the
 // place of 20 for 16 rows of 33 slots cut into 40 parts.)
 template <int D, bool F16>
 __global__ void __launch_bounds__(128) kv4_merge_kernel(const __grid_constant__ Kv4Args g) {
@@ -764,27 +784,30 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const __grid_constant__ 
   const int items = g.hkv * g.rb, slot = int(blockIdx.x) / items, item = int(blockIdx.x) % items;
   const int lane = threadIdx.x & 31, sub = lane / kLanes, col = lane % kLanes;
   const int head = item / g.rb, row0 = (item % g.rb) * 16;
-  const int r = (int(blockIdx.y) * 4 + int(threadIdx.x >> 5)) * kRows + sub;
+  const int warp = threadIdx.x >> 5, r = int(blockIdx.y) * kRows + sub;
+  __shared__ float4 quarter[3][32];
+  __shared__ float2 quarter_ml[3][32];
   const bool live = r < min(16, g.per - row0);
   pdl_enter();
-  const int before = g.before[slot], tiles = g.before[slot + 1] - before;
-  const int64_t total = int64_t(g.before[g.slots]) * items, n = min(int64_t(g.workers), total);
-  const int64_t t0 = int64_t(before) * items + int64_t(item) * tiles;
+  const int before = g.before[slot], units = g.before[slot + 1] - before;
+  const uint32_t share = kv4_share(uint32_t(g.before[g.slots]) * uint32_t(items), g.workers);
+  const uint32_t u0 = uint32_t(before) * uint32_t(items) + uint32_t(item) * uint32_t(units);
   int64_t w0 = 0;
   int parts = 0, first = 0;                                    // first: the part of worker w0 is its last, not its opening one
-  if (tiles > 0) {
-    w0 = kv4_worker(t0, total, n);
-    parts = int(kv4_worker(t0 + tiles - 1, total, n) - w0) + 1;
+  if (units > 0) {
+    w0 = (u0 + kKvItemCost) / share;
+    parts = int((u0 + units - 1) / share - w0) + 1;
     if (parts == 1) return;                                    // one worker held the whole item and wrote it
-    first = kv4_start(w0, total, n) < t0 ? 1 : 0;
+    first = uint32_t(w0) * share < u0 ? 1 : 0;
   }
   float top = -INFINITY, L = 0.f;
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
   const int rr = live ? r : 0;
-  for (int j0 = 0; j0 < parts; j0 += kLanes) {
+  const int j_lo = parts * warp / 4, j_hi = parts * (warp + 1) / 4;
+  for (int j0 = j_lo; j0 < j_hi; j0 += kLanes) {
     const int j = j0 + col;
     float m = -INFINITY, l = 0.f;
-    if (j < parts) {
+    if (j < j_hi) {
       const float2 ml = *reinterpret_cast<const float2 *>(g.part_ml + ((2 * (w0 + j) + (j == 0 ? first : 0)) * 16 + rr) * 2);
       m = ml.x, l = ml.y;
     }
@@ -800,7 +823,7 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const __grid_constant__ 
     L = L * back + part;
     O.x *= back, O.y *= back, O.z *= back, O.w *= back;
     top = now;
-    const int here = min(kLanes, parts - j0);
+    const int here = min(kLanes, j_hi - j0);
 #pragma unroll 8
     for (int k = 0; k < here; ++k) {
       const float w = __shfl_sync(0xffffffffu, e, k, kLanes);
@@ -809,7 +832,19 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const __grid_constant__ 
       O.x = fmaf(o.x, w, O.x), O.y = fmaf(o.y, w, O.y), O.z = fmaf(o.z, w, O.z), O.w = fmaf(o.w, w, O.w);
     }
   }
-  if (!live) return;
+  if (warp > 0) quarter[warp - 1][lane] = O, quarter_ml[warp - 1][lane] = make_float2(top, L);
+  __syncthreads();
+  if (warp > 0 || !live) return;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    const float4 o = quarter[k][lane];
+    const float2 ml = quarter_ml[k][lane];
+    const float now = fmaxf(top, ml.x);
+    const float a = now == top ? 1.f : ex2_fast(top - now), b = now == ml.x ? 1.f : ex2_fast(ml.x - now);   // equal: both may be -inf
+    L = L * a + ml.y * b;
+    O.x = O.x * a + o.x * b, O.y = O.y * a + o.y * b, O.z = O.z * a + o.z * b, O.w = O.w * a + o.w * b;
+    top = now;
+  }
   const float inv = top == -INFINITY && L == 0.f ? 0.f : 1.f / L;
   *reinterpret_cast<uint2 *>(g.b + slot * g.b_row + int64_t(head * g.per + row0 + r) * g.b_head + 4 * col) =
       make_uint2(pack_16x2<F16>(O.x * inv, O.y * inv), pack_16x2<F16>(O.z * inv, O.w * inv));
@@ -828,11 +863,11 @@ int64_t kv4_workspace(const ptsim_desc &d, int sm_count) {
 template <int D, int NG, int NT, bool F16>
 static int run_kv4_attn(const Kv4Args &g, const LaunchCtx &c) {
   constexpr auto kern = kv4_attn_kernel<D, NG, NT, F16>;
-  constexpr int fixed = kKvWarps * kKvStages * (kKvTile * (D + 8 * NG) + 12) + 16;
-  PTSIM_CUDA((smem_limit_once<kern>(fixed + 4 * (PTSIM_KV4_SLOTS + 1), c.device)));
-  PTSIM_CUDA(launch_pdl(kern, dim3(unsigned(g.workers / kKvWarps)), dim3(kKvWarps * 32), fixed + 4 * (g.slots + 1), c.stream, g));
+  constexpr int fixed = kKvWarps * kKvStages * (kKvTile * (D + 8 * NG) + 12) + 16;   // 6 bytes a slot follow
+  PTSIM_CUDA((smem_limit_once<kern>(fixed + 6 * (PTSIM_KV4_SLOTS + 1), c.device)));
+  PTSIM_CUDA(launch_pdl(kern, dim3(unsigned(g.workers / kKvWarps)), dim3(kKvWarps * 32), fixed + 6 * (g.slots + 1), c.stream, g));
   const int rows = g.per < 16 ? g.per : 16;
-  PTSIM_CUDA(launch_pdl(kv4_merge_kernel<D, F16>, dim3(unsigned(g.slots * g.hkv * g.rb), unsigned(ceil_div(rows * D, 512))), dim3(128), 0,
+  PTSIM_CUDA(launch_pdl(kv4_merge_kernel<D, F16>, dim3(unsigned(g.slots * g.hkv * g.rb), unsigned(ceil_div(rows * D, 128))), dim3(128), 0,
                         c.stream, g));
   return PTSIM_OK;
 }

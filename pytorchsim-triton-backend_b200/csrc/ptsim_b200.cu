@@ -182,7 +182,7 @@ static int check_kv4(const ptsim_desc &d) {
     if (q.hq < 1 || q.hq % q.hkv != 0 || q.hq > 65536)
       return fail(PTSIM_E_DESC, "4-bit cache attention with %lld query heads over %lld KV heads", (long long)q.hq, (long long)q.hkv);
     if (!(q.scale > 0.f && q.scale < INFINITY)) return fail(PTSIM_E_UNSUPPORTED, "4-bit cache attention with scale %g", q.scale);
-    if (q.slots * q.hkv * ceil_div(q.hq / q.hkv, 16) * ceil_div(q.max_pages * q.page_size, 64) >= (int64_t(1) << 31))
+    if (q.slots * q.hkv * ceil_div(q.hq / q.hkv, 16) * (ceil_div(q.max_pages * q.page_size, 64) + 1) >= (int64_t(1) << 31))
       return fail(PTSIM_E_UNSUPPORTED, "4-bit cache attention over more than 2^31 tiles of 64 keys");
   } else if ((rc = check_ints(d, q.cu_arg, q.slots + 1, "the table of token rows"))) {
     return rc;
