@@ -85,7 +85,7 @@ __device__ __forceinline__ int kv4_find(const Kv4Args &g, int t, int lane, int64
 // The pool page of position `pos` of slot s, or -1 (recorded) when the row or the pool does not hold it.
 __device__ __forceinline__ int kv4_page(const Kv4Args &g, int s, int64_t pos, int lane) {
   int page = -1;
-  if (pos >= 0 && pos / g.page_size < g.max_pages) page = g.table[int64_t(s) * g.max_pages + pos / g.page_size];
+  if (pos >= 0 && (pos >> g.page_log) < g.max_pages) page = g.table[int64_t(s) * g.max_pages + (pos >> g.page_log)];
   if (page >= 0 && page < g.pages) return page;
   if (lane == 0) record_status(PTSIM_E_OOB);
   return -1;
@@ -107,9 +107,9 @@ struct Kv4Lane {
     word = is_v ? (i & 7) * (D / 64) + (i >> 3) : (i & 3) * (D / 32) + (i >> 2);
   }
   // Byte offsets within a record of this lane's word and of its token's parameters.
-  __device__ __forceinline__ void place(int at, int page_size, int *code, int *par) const {
-    const int bs = page_size < 32 ? page_size : 32;
-    const int base = (at / bs) * (bs * (D + 8 * NG)), t = at % bs;
+  __device__ __forceinline__ void place(int at, int page_log, int *code, int *par) const {
+    const int bs_log = min(page_log, 5), bs = 1 << bs_log;
+    const int base = (at >> bs_log) * (bs * (D + 8 * NG)), t = at & (bs - 1);
     const int r = is_v ? (t & ~7) | ((t & 1) << 2) | ((t >> 1) & 3) : t;
     const int w = is_v && D == 128 && (r & 2) ? word ^ 8 : word;
     *code = base + (is_v ? bs * (D / 2) : 0) + r * (D / 2) + w * 4;
@@ -117,117 +117,175 @@ struct Kv4Lane {
   }
 };
 
-// One (token, head) per D/4 lanes: eight values a lane, their group's minimum and maximum by shuffles.
-template <int D, int NG, bool F16>
+// Minimum of the halves of a and b, a NaN where either is one.
+template <bool F16>
+__device__ __forceinline__ uint32_t min_16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (F16) asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// (minimum, -maximum) of two words' four values, as a pair.
+template <bool F16>
+__device__ __forceinline__ uint32_t extremes(uint32_t w0, uint32_t w1) {
+  const uint32_t lo = min_16x2<F16>(w0, w1), hi = min_16x2<F16>(w0 ^ 0x80008000u, w1 ^ 0x80008000u);
+  return min_16x2<F16>(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
+}
+
+// Eight values (two runs of four, a scale and a minimum for each) to codes, nibble e the e-th value.  rint of the fp32
+// quotient (x - mn) / step is the code; the quotient by the reciprocal is within 2^-18 of it, so the two round alike unless it
+// lies that near to a half, and then the division is carried out.  A float plus 1.5 * 2^23 is rounded to an integer in its low bits.
+template <bool F16>
+__device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], const float (&step)[2], const float (&mn)[2]) {
+  constexpr float kMagic = 12582912.f;
+  uint32_t word = 0;
+  float y[8], odd = 0.f;
+  const float r0 = step[0] > 0.f ? __frcp_rn(step[0]) : 0.f, r1 = step[1] > 0.f ? __frcp_rn(step[1]) : 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    y[e] = (e & 1 ? hi_f32<F16>(w[e >> 1]) : lo_f32<F16>(w[e >> 1])) - mn[e >> 2];
+    const float r = e < 4 ? r0 : r1, t = fminf(fmaf(y[e], r, kMagic), kMagic + 15.f);
+    odd = fmaxf(odd, fabsf(fmaf(y[e], r, kMagic - t)));      // distance from the code; past 0.5 where it was clamped
+    word += __float_as_uint(t) << (4 * e);
+  }
+  constexpr uint32_t base = 0x4b400000u;
+  word -= base + (base << 4) + (base << 8) + (base << 12) + (base << 16) + (base << 20) + (base << 24) + (base << 28);
+  // Near a half, clamped, or a quotient that is no number (0 * infinity of a step below 2^-126).
+  if (!(odd < 0.49999f)) {
+    word = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float q = rintf(__fdiv_rn(y[e], step[e >> 2]));
+      word |= uint32_t(fminf(fmaxf(q, 0.f), 15.f)) << (4 * e);
+    }
+  }
+  return word & ((step[0] > 0.f ? 0xffffu : 0u) | (step[1] > 0.f ? 0xffff0000u : 0u));
+}
+
+// One (token, head) per D / 4 lanes, eight values a lane, `HS` steps of 128 / D heads a warp: their loads are issued before the
+// token's place is looked up, so a warp waits for the two once.  Extremes are packed 16-bit minima of x and -x, one shuffle a step.
+template <int D, int NG, bool F16, int HS>
 __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ Kv4Args g, uint8_t *pool) {
-  constexpr int kLanes = D / 4, kHeads = 32 / kLanes;   // heads a warp takes at once
+  constexpr int kLanes = D / 4, kHeads = 32 / kLanes, kGroup = D / NG;
   const int lane = threadIdx.x & 31;
-  const int hsteps = (g.hkv + kHeads - 1) / kHeads;
-  const int64_t unit = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int t = int(unit / hsteps), h = int(unit % hsteps) * kHeads + lane / kLanes;
+  const uint32_t per_token = uint32_t(g.hkv + kHeads * HS - 1) / uint32_t(kHeads * HS);   // warps of a token
+  const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5), t = unit / per_token;
+  const int h0 = int(unit - t * per_token) * (kHeads * HS) + lane / kLanes;
   pdl_enter();
-  if (t >= g.tokens) return;
+  if (t >= uint32_t(g.tokens)) return;
   const Kv4Lane<D, NG> me(lane);
-  const bool live = h < g.hkv;
-  uint2 x0 = make_uint2(0, 0), x1 = x0;
-  if (live) {
-    const uint16_t *src = me.is_v ? g.b + t * g.b_row + h * g.b_head : g.a + t * g.a_row + h * g.a_head;
-    x0 = *reinterpret_cast<const uint2 *>(src + me.d0);
-    x1 = *reinterpret_cast<const uint2 *>(src + me.d1);
+  const uint16_t *src = me.is_v ? g.b + t * g.b_row : g.a + t * g.a_row;
+  const int64_t step_h = me.is_v ? g.b_head : g.a_head;
+  uint32_t w[HS][4];
+#pragma unroll
+  for (int i = 0; i < HS; ++i) {
+    const int h = h0 + i * kHeads;
+    uint2 x0 = make_uint2(0, 0), x1 = x0;
+    if (h < g.hkv) {
+      x0 = *reinterpret_cast<const uint2 *>(src + h * step_h + me.d0);
+      x1 = *reinterpret_cast<const uint2 *>(src + h * step_h + me.d1);
+    }
+    w[i][0] = x0.x, w[i][1] = x0.y, w[i][2] = x1.x, w[i][3] = x1.y;
   }
   int64_t pos = 0;
-  const int slot = kv4_find(g, t, lane, &pos);
+  const int slot = kv4_find(g, int(t), lane, &pos);
   if (slot < 0) return;
   const int page = kv4_page(g, slot, pos, lane);
   if (page < 0) return;
-  const float x[8] = {lo_f32<F16>(x0.x), hi_f32<F16>(x0.x), lo_f32<F16>(x0.y), hi_f32<F16>(x0.y),
-                      lo_f32<F16>(x1.x), hi_f32<F16>(x1.x), lo_f32<F16>(x1.y), hi_f32<F16>(x1.y)};
-  // Extremes of the lane's two runs of four; one group but for V in groups of 32.
-  float mn[2], mx[2];
+  int code_at, par_at;
+  me.place(int(pos) & ((1 << g.page_log) - 1), g.page_log, &code_at, &par_at);
+  uint8_t *rec = pool + int64_t(page) * g.hkv * g.record;
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    mn[r] = nan_min(nan_min(x[4 * r], x[4 * r + 1]), nan_min(x[4 * r + 2], x[4 * r + 3]));
-    mx[r] = nan_max(nan_max(x[4 * r], x[4 * r + 1]), nan_max(x[4 * r + 2], x[4 * r + 3]));
-  }
-  constexpr int kGroup = D / NG;
-  if (kGroup > 32 || !me.is_v) {
-    mn[0] = mn[1] = nan_min(mn[0], mn[1]);
-    mx[0] = mx[1] = nan_max(mx[0], mx[1]);
-  }
-  // Lanes of a group: group / 8 consecutive ones (V in groups of 32: all eight of its 64 values' lanes, by run).
+  for (int i = 0; i < HS; ++i) {
+    const int h = h0 + i * kHeads;
+    // (minimum, -maximum) of the lane's two runs of four; one group but for V in groups of 32.
+    uint32_t m0 = extremes<F16>(w[i][0], w[i][1]), m1 = extremes<F16>(w[i][2], w[i][3]);
+    const uint32_t both = min_16x2<F16>(m0, m1);
+    if (kGroup > 32 || !me.is_v) m0 = m1 = both;
+    // Lanes of a group: group / 8 consecutive ones (V in groups of 32: the eight lanes of its 64 values, by run).
 #pragma unroll
-  for (int s = 1; s < (kGroup > 64 ? 16 : 8); s *= 2)
+    for (int s = 1; s < (kGroup > 64 ? 16 : 8); s *= 2) {
+      const uint32_t a = min_16x2<F16>(m0, __shfl_xor_sync(0xffffffffu, m0, s));
+      const uint32_t b = kGroup > 32 ? a : min_16x2<F16>(m1, __shfl_xor_sync(0xffffffffu, m1, s));
+      if (kGroup > 32 || s < 4 || me.is_v) m0 = a, m1 = b;
+    }
+    float step[2], mn[2];
+    uint32_t par[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float a = nan_min(mn[r], __shfl_xor_sync(0xffffffffu, mn[r], s));
-      const float b = nan_max(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], s));
-      if (kGroup > 32 || s < 4 || me.is_v) mn[r] = a, mx[r] = b;
+      const uint32_t m = r ? m1 : m0;
+      mn[r] = lo_f32<F16>(m);
+      const float half = hi_f32<F16>(m) * -0.5f - mn[r] * 0.5f;           // half the range: the range itself could overflow
+      const bool fine = half < INFINITY;                                  // false for NaN too
+      par[r] = fine ? pack_16x2<F16>(__fdiv_rn(half, 7.5f), mn[r]) : (F16 ? 0x7e007e00u : 0x7fc07fc0u);   // the minimum is exact
+      step[r] = fine ? lo_f32<F16>(par[r]) : 0.f;                         // a group that is no number: codes 0
     }
-  uint32_t word = 0, par[2];
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const float half = mx[r] * 0.5f - mn[r] * 0.5f;           // halves: the range itself could overflow
-    const bool fine = half < INFINITY;                        // false for NaN too
-    const uint32_t s16 = pack_16x2<F16>(__fdiv_rn(half, 7.5f), mn[r]);   // (scale, minimum); the minimum is exact
-    const float step = lo_f32<F16>(s16);
-    par[r] = fine ? s16 : (F16 ? 0x7e007e00u : 0x7fc07fc0u);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float q = rintf(__fdiv_rn(x[4 * r + e] - mn[r], step));
-      const uint32_t code = fine && step > 0.f ? uint32_t(fminf(fmaxf(q, 0.f), 15.f)) : 0u;
-      const int d = 4 * r + e;                                // K: nibble (d / 2) + 4 (d % 2); V: run r, place e
-      word |= code << (4 * (me.is_v ? d : (d >> 1) + 4 * (d & 1)));
+    uint32_t word = quantise8<F16>(w[i], step, mn);
+    if (!me.is_v) {                                                       // K: value d in nibble d / 2 + 4 (d % 2)
+      const uint32_t x = (word ^ (word >> 4)) & 0x00f000f0u;
+      word = __byte_perm(word ^ x ^ (x << 4), 0, 0x3120);
     }
+    if (h >= g.hkv) continue;
+    uint8_t *to = rec + h * g.record;
+    *reinterpret_cast<uint32_t *>(to + code_at) = word;
+    // The first lane of each group writes its parameters.
+    if (me.d0 % kGroup == 0) *reinterpret_cast<uint32_t *>(to + par_at + 4 * (me.d0 / kGroup)) = par[0];
+    if (kGroup == 32 && me.is_v && (me.i & 7) == 0) *reinterpret_cast<uint32_t *>(to + par_at + 4 * (me.d1 / kGroup)) = par[1];
   }
-  if (!live) return;
-  int code_at, par_at;
-  me.place(int(pos % g.page_size), g.page_size, &code_at, &par_at);
-  uint8_t *rec = pool + (int64_t(page) * g.hkv + h) * g.record;
-  *reinterpret_cast<uint32_t *>(rec + code_at) = word;
-  // The first lane of each group writes its parameters.
-  if (me.d0 % kGroup == 0) *reinterpret_cast<uint32_t *>(rec + par_at + 4 * (me.d0 / kGroup)) = par[0];
-  if (kGroup == 32 && me.is_v && (me.i & 7) == 0) *reinterpret_cast<uint32_t *>(rec + par_at + 4 * (me.d1 / kGroup)) = par[1];
 }
 
-template <int D, int NG, bool F16>
+template <int D, int NG, bool F16, int HS>
 __global__ void __launch_bounds__(256) kv4_load_kernel(const __grid_constant__ Kv4Args g) {
   constexpr int kLanes = D / 4, kHeads = 32 / kLanes, kGroup = D / NG;
   const int lane = threadIdx.x & 31;
-  const int hsteps = (g.hkv + kHeads - 1) / kHeads;
-  const int64_t unit = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int t = int(unit / hsteps), h = int(unit % hsteps) * kHeads + lane / kLanes;
+  const uint32_t per_token = uint32_t(g.hkv + kHeads * HS - 1) / uint32_t(kHeads * HS);
+  const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5), t = unit / per_token;
+  const int h0 = int(unit - t * per_token) * (kHeads * HS) + lane / kLanes;
   pdl_enter();
-  if (t >= g.tokens) return;
+  if (t >= uint32_t(g.tokens)) return;
   int64_t pos = 0;
-  const int slot = kv4_find(g, t, lane, &pos);
-  if (slot < 0 || h >= g.hkv) return;
+  const int slot = kv4_find(g, int(t), lane, &pos);
+  if (slot < 0) return;
   const int page = kv4_page(g, slot, pos, lane);
   const Kv4Lane<D, NG> me(lane);
-  uint32_t word = 0, p0 = 0, p1 = 0;                          // a page outside the pool reads as zeros
-  if (page >= 0) {
-    int code_at, par_at;
-    me.place(int(pos % g.page_size), g.page_size, &code_at, &par_at);
-    const uint8_t *rec = g.pool + (int64_t(page) * g.hkv + h) * g.record;
-    word = *reinterpret_cast<const uint32_t *>(rec + code_at);
-    p0 = *reinterpret_cast<const uint32_t *>(rec + par_at + 4 * (me.d0 / kGroup));
-    p1 = *reinterpret_cast<const uint32_t *>(rec + par_at + 4 * (me.d1 / kGroup));
-  }
-  uint32_t out[4];
+  int code_at, par_at;
+  me.place(int(pos) & ((1 << g.page_log) - 1), g.page_log, &code_at, &par_at);
+  const uint8_t *rec = g.pool + int64_t(max(page, 0)) * g.hkv * g.record;
+  uint32_t word[HS], p0[HS], p1[HS];
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    const float s = lo_f32<F16>(r ? p1 : p0), mn = hi_f32<F16>(r ? p1 : p0);
-    float y[4];
+  for (int i = 0; i < HS; ++i) {
+    const int h = h0 + i * kHeads;
+    word[i] = p0[i] = p1[i] = 0;                              // a page outside the pool reads as zeros
+    if (page < 0 || h >= g.hkv) continue;
+    const uint8_t *at = rec + h * g.record;
+    word[i] = *reinterpret_cast<const uint32_t *>(at + code_at);
+    p0[i] = *reinterpret_cast<const uint32_t *>(at + par_at + 4 * (me.d0 / kGroup));
+    p1[i] = kGroup > 32 ? p0[i] : *reinterpret_cast<const uint32_t *>(at + par_at + 4 * (me.d1 / kGroup));
+  }
+  uint16_t *dst = me.is_v ? g.b + t * g.b_row : g.a + t * g.a_row;
+  const int64_t step_h = me.is_v ? g.b_head : g.a_head;
+#pragma unroll
+  for (int i = 0; i < HS; ++i) {
+    const int h = h0 + i * kHeads;
+    uint32_t x = word[i];
+    if (!me.is_v) {                                           // K: nibble d / 2 + 4 (d % 2) to nibble d
+      x = __byte_perm(x, 0, 0x3120);
+      const uint32_t y = (x ^ (x >> 4)) & 0x00f000f0u;
+      x ^= y ^ (y << 4);
+    }
+    uint32_t out[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int d = 4 * r + e;
-      y[e] = __fmaf_rn(s, float((word >> (4 * (me.is_v ? d : (d >> 1) + 4 * (d & 1)))) & 15u), mn);
+      const uint32_t par = e < 2 ? p0[i] : p1[i];
+      const float s = lo_f32<F16>(par), mn = hi_f32<F16>(par);
+      const float c0 = __uint_as_float(((x >> (8 * e)) & 15u) | 0x4b000000u) - 8388608.f;
+      const float c1 = __uint_as_float(((x >> (8 * e + 4)) & 15u) | 0x4b000000u) - 8388608.f;
+      out[e] = pack_16x2<F16>(__fmaf_rn(s, c0, mn), __fmaf_rn(s, c1, mn));
     }
-    out[2 * r] = pack_16x2<F16>(y[0], y[1]);
-    out[2 * r + 1] = pack_16x2<F16>(y[2], y[3]);
+    if (h >= g.hkv) continue;
+    *reinterpret_cast<uint2 *>(dst + h * step_h + me.d0) = make_uint2(out[0], out[1]);
+    *reinterpret_cast<uint2 *>(dst + h * step_h + me.d1) = make_uint2(out[2], out[3]);
   }
-  uint16_t *dst = me.is_v ? g.b + t * g.b_row + h * g.b_head : g.a + t * g.a_row + h * g.a_head;
-  *reinterpret_cast<uint2 *>(dst + me.d0) = make_uint2(out[0], out[1]);
-  *reinterpret_cast<uint2 *>(dst + me.d1) = make_uint2(out[2], out[3]);
 }
 
 // -------------------------------------------------------------------------------------------------------------------
@@ -876,13 +934,16 @@ template <int D, int NG, bool F16>
 static int run_kv4(const ptsim_desc &d, Kv4Args &g, uint8_t *pool, const LaunchCtx &c) {
   if (d.kind == PTSIM_KIND_ATTN_KV4)
     return d.p.kv4.hq / d.p.kv4.hkv <= 8 ? run_kv4_attn<D, NG, 1, F16>(g, c) : run_kv4_attn<D, NG, 2, F16>(g, c);
+  // A warp takes four steps of heads where that leaves every SM 32 warps or more, else one, so that a decode step's few tokens
+  // spread.
   constexpr int kHeads = 128 / D;
-  const int64_t units = g.tokens * ceil_div(g.hkv, kHeads);
-  const dim3 grid(unsigned(ceil_div(units, 8)));
+  const int64_t four = g.tokens * ceil_div(g.hkv, 4 * kHeads), one = g.tokens * ceil_div(g.hkv, kHeads);
+  const bool many = four >= int64_t(c.sm_count) * 32;
+  const dim3 grid(unsigned(ceil_div(many ? four : one, 8)));
   if (d.kind == PTSIM_KIND_KV4_STORE)
-    PTSIM_CUDA(launch_pdl(kv4_store_kernel<D, NG, F16>, grid, dim3(256), 0, c.stream, g, pool));
+    PTSIM_CUDA(launch_pdl(many ? kv4_store_kernel<D, NG, F16, 4> : kv4_store_kernel<D, NG, F16, 1>, grid, dim3(256), 0, c.stream, g, pool));
   else
-    PTSIM_CUDA(launch_pdl(kv4_load_kernel<D, NG, F16>, grid, dim3(256), 0, c.stream, g));
+    PTSIM_CUDA(launch_pdl(many ? kv4_load_kernel<D, NG, F16, 4> : kv4_load_kernel<D, NG, F16, 1>, grid, dim3(256), 0, c.stream, g));
   return PTSIM_OK;
 }
 
