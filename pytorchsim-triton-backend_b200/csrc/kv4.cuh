@@ -132,34 +132,58 @@ __device__ __forceinline__ uint32_t extremes(uint32_t w0, uint32_t w1) {
   return min_16x2<F16>(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
 }
 
+// half / 7.5 correctly rounded: the quotient by the rounded reciprocal, corrected by its exact remainder (Markstein's
+// method, for a divisor known in advance).
+__device__ __forceinline__ float over_seven_and_a_half(float half) {
+  constexpr float r = 1.f / 7.5f;
+  const float q = half * r;
+  return fmaf(fmaf(-7.5f, q, half), r, q);
+}
+
 // Eight values (two runs of four, a scale and a minimum for each) to codes, nibble e the e-th value.  rint of the fp32
-// quotient (x - mn) / step is the code; the quotient by the reciprocal is within 2^-18 of it, so the two round alike unless it
-// lies that near to a half, and then the division is carried out.  A float plus 1.5 * 2^23 is rounded to an integer in its low bits.
+// quotient y / step, y = x - mn, is the code.  The quotient by the reciprocal is within 2^-18 of it, so the two round alike unless it
+// lies that near to a half, n + 1/2 say, as every 400th value of a bf16 grid does exactly; then y is compared with
+// (n + 1/2) step, which fp32 holds exactly (11 bits times 5), and a tie goes to the even code.  (Only a quotient of 1/2 + 2^-25 would
+// be rounded to the tie and is not one; it takes a y of 24 bits.)  A float plus 1.5 * 2^23 is rounded to an integer in its low bits.
 template <bool F16>
 __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], const float (&step)[2], const float (&mn)[2]) {
-  constexpr float kMagic = 12582912.f;
+  // Steps from kTiny on are rounded by at most 2^-9 of themselves: no quotient passes 15.5, and the reciprocal is a normal number.
+  constexpr float kMagic = 12582912.f, kTiny = F16 ? 6.103515625e-5f : 1e-30f;
   uint32_t word = 0;
-  float y[8], odd = 0.f;
-  const float r0 = step[0] > 0.f ? __frcp_rn(step[0]) : 0.f, r1 = step[1] > 0.f ? __frcp_rn(step[1]) : 0.f;
+  float y[8], d[8], n[8], r[2], odd = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    y[e] = (e & 1 ? hi_f32<F16>(w[e >> 1]) : lo_f32<F16>(w[e >> 1])) - mn[e >> 2];
-    const float r = e < 4 ? r0 : r1, t = fminf(fmaf(y[e], r, kMagic), kMagic + 15.f);
-    odd = fmaxf(odd, fabsf(fmaf(y[e], r, kMagic - t)));      // distance from the code; past 0.5 where it was clamped
-    word += __float_as_uint(t) << (4 * e);
+  for (int k = 0; k < 2; ++k) {
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r[k]) : "f"(step[k]));
+    if (step[k] < kTiny) r[k] = 0.f;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    const float m = -mn[e >> 2], k = r[e >> 2];
+    const float2 magic = make_float2(kMagic, kMagic), y2 = __fadd2_rn(make_float2(lo_f32<F16>(w[e >> 1]), hi_f32<F16>(w[e >> 1])), make_float2(m, m));
+    const float2 t2 = __ffma2_rn(y2, make_float2(k, k), magic), n2 = __fadd2_rn(t2, make_float2(-kMagic, -kMagic));
+    const float2 d2 = __ffma2_rn(y2, make_float2(k, k), make_float2(-n2.x, -n2.y));
+    y[e] = y2.x, y[e + 1] = y2.y, n[e] = n2.x, n[e + 1] = n2.y, d[e] = d2.x, d[e + 1] = d2.y;
+    odd = fmaxf(odd, fmaxf(fabsf(d2.x), fabsf(d2.y)));
+    word += (__float_as_uint(t2.x) << (4 * e)) + (__float_as_uint(t2.y) << (4 * e + 4));
   }
   constexpr uint32_t base = 0x4b400000u;
   word -= base + (base << 4) + (base << 8) + (base << 12) + (base << 16) + (base << 20) + (base << 24) + (base << 28);
-  // Near a half, clamped, or a quotient that is no number (0 * infinity of a step below 2^-126).
-  if (!(odd < 0.49999f)) {
+  // Also one value after the other: a step too small for its reciprocal, and a run without one (a constant, or no number).
+  if (odd > 0.49999f || step[0] < kTiny || step[1] < kTiny) {
     word = 0;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float q = rintf(__fdiv_rn(y[e], step[e >> 2]));
-      word |= uint32_t(fminf(fmaxf(q, 0.f), 15.f)) << (4 * e);
+      const float s = step[e >> 2];
+      float c = n[e];
+      if (fabsf(d[e]) > 0.49999f) {
+        const float below = d[e] > 0.f ? n[e] : n[e] - 1.f, tie = (below + 0.5f) * s;
+        c = y[e] > tie || (y[e] == tie && (int(below) & 1)) ? below + 1.f : below;
+      }
+      if (s < kTiny) c = s > 0.f ? rintf(__fdiv_rn(y[e], s)) : 0.f;
+      word |= uint32_t(fminf(fmaxf(c, 0.f), 15.f)) << (4 * e);
     }
   }
-  return word & ((step[0] > 0.f ? 0xffffu : 0u) | (step[1] > 0.f ? 0xffff0000u : 0u));
+  return word;
 }
 
 // One (token, head) per D / 4 lanes, eight values a lane, `HS` steps of 128 / D heads a warp: their loads are issued before the
@@ -217,7 +241,7 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ 
       mn[r] = lo_f32<F16>(m);
       const float half = hi_f32<F16>(m) * -0.5f - mn[r] * 0.5f;           // half the range: the range itself could overflow
       const bool fine = half < INFINITY;                                  // false for NaN too
-      par[r] = fine ? pack_16x2<F16>(__fdiv_rn(half, 7.5f), mn[r]) : (F16 ? 0x7e007e00u : 0x7fc07fc0u);   // the minimum is exact
+      par[r] = fine ? pack_16x2<F16>(over_seven_and_a_half(half), mn[r]) : (F16 ? 0x7e007e00u : 0x7fc07fc0u);   // the minimum is exact
       step[r] = fine ? lo_f32<F16>(par[r]) : 0.f;                         // a group that is no number: codes 0
     }
     uint32_t word = quantise8<F16>(w[i], step, mn);
