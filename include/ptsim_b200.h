@@ -316,7 +316,7 @@ typedef struct ptsim_itab_params {
  * x_arg (q, k, v may be parts of one argument); offsets and strides are multiples of 8 elements.  A table that
  * descends or leaves the tokens records PTSIM_E_OOB and its sequence is skipped.  bf16 or fp16 throughout; dim 64 or
  * 128; scale > 0, scores scale q.k below 2^20; at most PTSIM_PACKED_SEQS sequences.  One partition unit. */
-#define PTSIM_PACKED_SEQS 4096
+#define PTSIM_PACKED_SEQS 1024
 typedef struct ptsim_pattn_params {
   int64_t q_tokens, k_tokens, seqs, hq, hkv, dim;
   int64_t q_off, q_row, q_head, k_off, k_row, k_head, v_off, v_row, v_head, o_off, o_row, o_head;

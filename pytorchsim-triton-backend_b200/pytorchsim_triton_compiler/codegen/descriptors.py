@@ -155,7 +155,7 @@ class ItabParams(C.Structure):
                 ("maps", Map * ITAB_MAPS), ("out", ItabOut * ITAB_OUTS), ("code", IInsn * MAX_ICODE)]
 
 
-PACKED_SEQS, KV4_SLOTS, PAGES_IDS = 4096, 4096, 1024   # PTSIM_PACKED_SEQS, PTSIM_KV4_SLOTS, PTSIM_PAGES_IDS
+PACKED_SEQS, KV4_SLOTS, PAGES_IDS = 1024, 4096, 1024   # PTSIM_PACKED_SEQS, PTSIM_KV4_SLOTS, PTSIM_PAGES_IDS
 
 
 class PackedAttnParams(C.Structure):
