@@ -16,6 +16,7 @@ class Graph:
         self.device = torch.device(device)
         self.buffers = {}
         self.steps = []          # (name, blob, [buffer names], workspace, units, owners)
+        self._prepared = {}      # step index -> (pointers, native.Prepared over them)
         self.cuda_graph = None
 
     def buffer(self, name, numel, dtype, init=None):
@@ -73,20 +74,29 @@ class Graph:
         if self.cuda_graph is not None and stream is None:
             self.cuda_graph.replay()
         else:
-            with torch.cuda.device(self.device):
-                for step in self.steps:
-                    self._launch(step, s.cuda_stream)
+            ptr = s.cuda_stream
+            if torch.cuda.current_device() == (self.device.index or 0):
+                for i in range(len(self.steps)):
+                    self._launch(i, ptr)
+            else:
+                with torch.cuda.device(self.device):
+                    for i in range(len(self.steps)):
+                        self._launch(i, ptr)
         if sync:
             native.sync(s.cuda_stream)
 
-    def _launch(self, step, stream):
-        name, blob, bufs, ws, units, owners = step
+    def _launch(self, i, stream):
+        name, blob, bufs, ws, units, owners = self.steps[i]
         ptrs = [self.buffers[b].data_ptr() for b in bufs]
-        wp, wn = (ws.data_ptr(), ws.numel()) if ws is not None else (0, 0)
-        if owners is None:
-            native.launch(blob, ptrs, 0, units, wp, wn, stream)
-        else:
+        if owners is not None:
+            wp, wn = (ws.data_ptr(), ws.numel()) if ws is not None else (0, 0)
             native.launch_rows_to_owners(blob, ptrs, 0, units, owners[0], owners[1], wp, wn, stream)
+            return
+        held = self._prepared.get(i)
+        if held is None or held[0] != ptrs:
+            wp, wn = (ws.data_ptr(), ws.numel()) if ws is not None else (0, 0)
+            held = self._prepared[i] = (ptrs, native.Prepared(blob, ptrs, units, wp, wn))
+        held[1].run(stream)
 
     def capture(self):
         """Capture the launch sequence into a CUDA graph (replayed by run())."""
@@ -98,8 +108,8 @@ class Graph:
         s.wait_stream(torch.cuda.current_stream(self.device))
         with torch.cuda.stream(s):
             with torch.cuda.graph(g, stream=s):
-                for step in self.steps:
-                    self._launch(step, s.cuda_stream)
+                for i in range(len(self.steps)):
+                    self._launch(i, s.cuda_stream)
         torch.cuda.current_stream(self.device).wait_stream(s)
         self.cuda_graph = g
         return g

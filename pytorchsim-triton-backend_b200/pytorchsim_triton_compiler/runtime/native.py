@@ -161,6 +161,22 @@ def launch(blob, ptrs, lo, hi, workspace=0, workspace_bytes=0, stream=0):
                             int(workspace_bytes), C.c_void_p(int(stream) or None)))
 
 
+class Prepared:
+    """A launch of units [0, units) of descriptor `blob` with its arguments converted once, for a caller that repeats it
+    over the same device pointers: run(stream) is ptsim_launch alone."""
+
+    def __init__(self, blob, ptrs, units, workspace=0, workspace_bytes=0):
+        self._fn = load().ptsim_launch
+        n = len(ptrs)
+        self._args = (_desc_buffer(blob), len(blob), (C.c_void_p * max(1, n))(*[int(p) or None for p in ptrs]), n, 0, int(units),
+                      int(workspace) or None, int(workspace_bytes))
+
+    def run(self, stream=0):
+        rc = self._fn(*self._args, stream or None)
+        if rc:
+            _check(rc)
+
+
 def launch_reduce_noalloc(blob, ptrs, stream=0):
     """Enqueue a whole-tensor reduction of `blob` with the library's own 4 KiB static scratch: for callers
     that cannot allocate device memory.  Calls that overlap on the GPU share that scratch and race."""
