@@ -336,7 +336,7 @@ typedef struct ptsim_pattn_params {
  *   c = d % 32 / 4, c ^ 4 for dim 128 where r & 2, nibble d % 4 + 4 (d % 64 / 32).
  *
  * KV4_STORE: token rows cu[s] .. cu[s + 1] of a (keys) and b (values) become the last tokens of slot s, which holds
- * lens[s] tokens with them (its pages are in the table already).  KV4_LOAD: the reverse, the last cu[s + 1] - cu[s]
+ * lens[s] tokens with them (its pages are in the table already; a page that is written is held by that slot alone).  KV4_LOAD: the reverse, the last cu[s + 1] - cu[s]
  * tokens of slot s into rows of a and b, scale * code + minimum in fp32 rounded to their type; rows of no slot are
  * left alone.  ATTN_KV4: a = q, b = o,
  * rows of one token per slot: query head h of slot s attends over the lens[s] cached tokens of KV head h / (hq / hkv); a

@@ -65,8 +65,10 @@ __device__ __forceinline__ int4 pages_refs4(const PagesArgs &g, int p) {
 
 __global__ void __launch_bounds__(kPagesThreads) pages_plan_kernel(const __grid_constant__ PagesArgs g) {
   __shared__ int ids[PTSIM_PAGES_IDS], aux[PTSIM_PAGES_IDS], base[PTSIM_PAGES_IDS], first[PTSIM_PAGES_IDS];
-  __shared__ int sums[33];
+  __shared__ int sums[33], refused;
+  __shared__ unsigned long long asked;
   const int i = threadIdx.x;
+  if (i == 0) refused = 0, asked = 0;
   pdl_enter();
   if (g.op == PTSIM_PAGES_COMPACT) {
     // Used pages, then the k-th hole below their number and the k-th used page from it on.
@@ -115,6 +117,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_plan_kernel(const __grid_
 
   // Checks; the pages entry i asks for.
   int code = 0, need = 0, len = 0;
+  int4 ahead = pages_refs4(g, 4 * i);     // the first 4096 counts come in beside the lists
   if (i < g.n) {
     ids[i] = g.ids[i];
     aux[i] = g.aux[i];
@@ -141,16 +144,19 @@ __global__ void __launch_bounds__(kPagesThreads) pages_plan_kernel(const __grid_
     for (int j = 0; j < g.n && code == 0; ++j)
       if ((j < i && (grow ? ids[j] == a : aux[j] == b)) || (!grow && ids[j] == b)) code = PTSIM_E_ARGS;
   }
+  if (need > 0) atomicAdd(&asked, (unsigned long long)need);      // the scan's 32 bits could wrap
+  if (code) atomicOr(&refused, code == PTSIM_E_OOB ? 1 : code == PTSIM_E_ARGS ? 2 : 4);
   int total, found = 0;
-  const int at = block_scan(code ? 0 : need, sums, &total);
+  const int at = block_scan(code ? 0 : need, sums, &total);   // its barriers make `refused` everyone's
   if (i < g.n) base[i] = at;
-  const bool args = __syncthreads_or(code == PTSIM_E_ARGS), oob = __syncthreads_or(code == PTSIM_E_OOB);
-  bool short_ = __syncthreads_or(code == PTSIM_E_RESOURCE) || total > g.pages || total < 0;
+  const bool oob = refused & 1, args = refused & 2;
+  bool short_ = (refused & 4) || asked > (unsigned long long)g.pages;
   if (!args && !oob && !short_) {
     // The `total` lowest free pages, in order.
     for (int p0 = 0; p0 < g.pages && found < total; p0 += 4 * kPagesThreads) {
       const int p = p0 + 4 * i;
-      const int4 r = pages_refs4(g, p);
+      const int4 r = ahead;
+      if (p0 + 4 * kPagesThreads < g.pages) ahead = pages_refs4(g, p + 4 * kPagesThreads);
       const int c[4] = {r.x, r.y, r.z, r.w};
       int sum, k = found + block_scan((c[0] <= 0) + (c[1] <= 0) + (c[2] <= 0) + (c[3] <= 0), sums, &sum);
 #pragma unroll
@@ -208,7 +214,8 @@ __global__ void __launch_bounds__(256) pages_apply_kernel(const __grid_constant_
       int32_t *row = g.table + s * g.max_pages;
       for (int k = threadIdx.x; k < pages_held(g, len); k += 256) {
         const int p = row[k];
-        if (p >= live && p < g.pages) row[k] = g.remap[p];
+        if (p < 0 || p >= g.pages) record_status(PTSIM_E_OOB);
+        else if (p >= live) row[k] = g.remap[p];
       }
     }
   } else if (g.op == PTSIM_PAGES_FORK) {
@@ -282,7 +289,6 @@ int64_t pages_workspace(const ptsim_desc &d) {
 int launch_pages(const ptsim_desc &d, void *const *ptrs, void *ws, size_t ws_bytes, const LaunchCtx &c) {
   const ptsim_pages_params &p = d.p.pages;
   if (p.op != PTSIM_PAGES_COMPACT && p.n == 0) return PTSIM_OK;
-  if (p.pages == 0 || p.slots == 0) return PTSIM_OK;
   PagesArgs g;
   memset(&g, 0, sizeof(g));
   auto ints = [&](int arg) { return arg < 0 ? nullptr : static_cast<int32_t *>(ptrs[arg]); };

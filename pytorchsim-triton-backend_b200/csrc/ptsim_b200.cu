@@ -209,7 +209,7 @@ static int check_pages(const ptsim_desc &d) {
   if (rc || (rc = check_ints(d, q.refs_arg, q.pages, "the page counts"))) return rc;
   if (q.op != PTSIM_PAGES_COMPACT && (rc = check_ints(d, q.ids_arg, q.n, "the listed slots"))) return rc;
   if (q.op < PTSIM_PAGES_FREE && (rc = check_ints(d, q.aux_arg, q.n, "the second list"))) return rc;
-  if (q.slots == 0 && q.n > 0) return fail(PTSIM_E_DESC, "a page operation on a cache without slots");
+  if (q.slots < 1 || q.pages < 1 || q.max_pages < 1) return fail(PTSIM_E_DESC, "a page operation on a cache without slots or pages");
   return PTSIM_OK;
 }
 

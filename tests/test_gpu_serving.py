@@ -115,6 +115,35 @@ def test_packed_attention_with_cached_prefixes(ql, kl, dim, dtype):
         assert not o[q0[s]:q0[s] + hidden].any()
 
 
+# Averages of 768 keys (dim 128) and 4096 (dim 64) and more run two query tiles a CTA.
+@pytest.mark.parametrize("ql,kl,dim,dtype", [
+    ([1025, 3, 1400], [1025, 3, 1400], 128, "bfloat16"), ([257, 1, 128, 640], [2000, 900, 128, 641], 128, "float16"),
+    ([300, 129, 0, 5], [5000, 4300, 9000, 6], 64, "bfloat16"), ([1500], [800], 128, "bfloat16"), ([513, 256], [4096, 4351], 64, "float16")], ids=str)
+def test_packed_attention_of_long_sequences(ql, kl, dim, dtype):
+    q, k, v, q0, k0 = packed_case(ql, kl, 3, 1, dim, dtype, sum(kl))
+    o = torch.full_like(q, 7.0)
+    launch(B.attention_packed(q0[-1], len(ql), 3, 1, dim, dtype=dtype, k_tokens=k0[-1]), [q, k, v, ints(q0), ints(k0), o])
+    near(o, *dense(q, k, v, ql, kl, q0, k0, 1 / math.sqrt(dim)), DT[dtype])
+
+
+def test_packed_attention_of_long_sequences_is_blind_to_keys_it_does_not_see():
+    lens = [900, 1000, 800]
+    q, k, v, q0, k0 = packed_case(lens, lens, 2, 1, 128, "bfloat16", 21)
+    clean = [x.clone() for x in (q, k, v)]
+    at = q0[1] + 700                                      # in the second tile of its pair
+    v[at, 0, 3], v[at + 1, 0, 100] = float("nan"), -float("inf")
+    v[q0[1] - 1, 0, 7], k[q0[1] - 1, 0, 7] = float("inf"), float("nan")   # the last key of the first sequence
+    o = torch.zeros_like(q)
+    launch(B.attention_packed(q0[-1], 3, 2, 1), [q, k, v, ints(q0), o])
+    want, mag = dense(*clean, lens, lens, q0, k0, 1 / math.sqrt(128))
+    fine = torch.ones(q0[-1], dtype=torch.bool, device="cuda")
+    fine[q0[1] - 1] = False
+    fine[at:q0[2]] = False
+    near(o[fine], want[fine], mag[fine], torch.bfloat16)
+    assert o[q0[1] - 1].isnan().all() and o[at:q0[2], :, 3].isnan().all()
+    assert o[at, :, 100].isfinite().all() and bool((o[at + 1:at + 40, :, 100] == -math.inf).all())
+
+
 def test_packed_attention_leaves_rows_outside_every_sequence():
     lens = [100, 260]
     q, k, v, q0, k0 = packed_case(lens, lens, 4, 4, 128, "bfloat16", 5, gap=37, tail=90)
@@ -294,6 +323,57 @@ def test_store_writes_the_defined_bytes_and_load_reads_them(dim, page, group, hk
             row += 1
     assert len(bad) <= 8, f"{len(bad)} bytes differ from the definition"     # at most the two NaN pairs
     assert bool((got[0] == 0xA5).all())                                       # the other layer
+
+
+@pytest.mark.parametrize("dim,group,hkv,dtype,page", [(128, 64, 5, "bfloat16", 16), (128, 32, 4, "float16", 64), (64, 32, 3, "bfloat16", 32)])
+def test_store_of_many_tokens_is_the_store_of_few(dim, group, hkv, dtype, page):
+    """Several heads a warp (many tokens) and one (few) write the same bytes; the values are those of the definition."""
+    lens = [4000, 1, 5100, 777]
+    c, table, pool = cache_case(lens, dim, page, group, hkv, dtype, 3)
+    k, v = rows_of(sum(lens), c, 4)
+    cu, books = starts(lens), [ints(lens), ints(table)]
+    launch(B.kv4_store(c, sum(lens)), [k, v, ints(cu)] + books + [pool])
+    other, step = torch.full_like(pool, 0xA5), 500
+    for s, n in enumerate(lens):
+        for lo in range(0, n, step):
+            m = min(step, n - lo)
+            part = [0] * 4
+            part[s] = m
+            now = [lo + m if i == s else 0 for i in range(4)]
+            rows = slice(cu[s] + lo, cu[s] + lo + m)
+            launch(B.kv4_store(c, m), [k[rows], v[rows], ints(starts(part)), ints(now), ints(table), other])
+    assert torch.equal(pool, other)
+    kb, vb = torch.zeros_like(k), torch.zeros_like(v)
+    launch(B.kv4_load(c, sum(lens)), [ints(cu)] + books + [pool, kb, vb])
+    for got, x in ((kb, k), (vb, v)):
+        want = S.dequantised(x, group)
+        lim = torch.finfo(DT[dtype]).eps / 2 * want.abs() + 2.0 ** -24 * 64 + SMALLEST[DT[dtype]]
+        assert bool(((got.double() - want).abs() <= lim).all())
+
+
+def test_a_cache_past_four_gigabytes():
+    """Pages whose records lie past 2^32 bytes: written, read, attended to, and moved."""
+    pages, lens = 300000, [33, 20]
+    c = B.kv4_cache(slots=2, max_pages=3, pages=pages, hkv=8, dim=128, page_size=16, group=64)
+    assert c.pool_bytes > 5 << 30
+    pool = torch.empty(c.pool_bytes, dtype=torch.uint8, device="cuda")
+    table = [[pages - 1, 7, pages - 5], [pages - 2, 250000, -1]]
+    k, v = rows_of(53, c, 5)
+    q = torch.randn(2, 16, 128, generator=gen(6)).to(torch.bfloat16).cuda()
+    t, n, cu = ints(table), ints(lens), ints(starts(lens))
+    launch(B.kv4_store(c, 53), [k, v, cu, n, t, pool])
+    want, mag = cache_attention(q, k, v, lens, 64, 1 / math.sqrt(128))
+    o = torch.zeros_like(q)
+    launch(B.attention_kv4(c, 16), [q, n, t, pool, o])
+    near(o, want, mag, torch.bfloat16)
+    refs = torch.zeros(pages, dtype=torch.int32, device="cuda")
+    refs[[p for row in table for p in row if p >= 0]] = 1
+    launch(B.pages_compact(c), [t, n, refs, pool])
+    # used: 7, 250000, pages - 5, - 2, - 1; the k-th of those past 5 goes to the k-th free page below it
+    assert t.tolist() == [[4, 0, 2], [3, 1, -1]]
+    again = torch.zeros_like(q)
+    launch(B.attention_kv4(c, 16), [q, n, t, pool, again])
+    assert torch.equal(o, again)
 
 
 def test_store_and_load_skip_and_report_what_has_no_place():
@@ -734,14 +814,14 @@ def test_launch_tensors_can_be_captured():
     assert not a.refs.any() and not a.lens.any()
 
 
-@pytest.mark.parametrize("family", ["packed", "kv4"])
+@pytest.mark.parametrize("family", ["packed", "packed_long", "kv4"])
 def test_stalled_stage_times_out_and_device_stays_usable(family):
     """A withheld copy ends in PTSIM_E_TIMEOUT within the test's limit, and the next launch is right."""
-    if family == "packed":
-        lens = [600]
+    if family != "kv4":
+        lens = [600 if family == "packed" else 1600]
         q, k, v, q0, k0 = packed_case(lens, lens, 2, 1, 128, "bfloat16", 80)
         o = torch.zeros_like(q)
-        desc, ts, want = B.attention_packed(600, 1, 2, 1), [q, k, v, ints(q0), o], dense(q, k, v, lens, lens, q0, k0, 1 / math.sqrt(128))
+        desc, ts, want = B.attention_packed(lens[0], 1, 2, 1), [q, k, v, ints(q0), o], dense(q, k, v, lens, lens, q0, k0, 1 / math.sqrt(128))
     else:
         lens = [900]
         c, table, pool = cache_case(lens, 128, 16, 64, 1, "bfloat16", 81)

@@ -109,7 +109,7 @@ def test_cache_refusals_of_types():
     (lambda c: B.pages_grow(c, 2), dict(op=9), D.E_DESC), (lambda c: B.pages_grow(c, 2), dict(n=3), D.E_OOB),
     (lambda c: B.pages_grow(c, 2), dict(n=D.PAGES_IDS + 1), D.E_UNSUPPORTED), (lambda c: B.pages_grow(c, 2), dict(n=-1), D.E_DESC),
     (lambda c: B.pages_grow(c, 2), dict(pages=10), D.E_OOB), (lambda c: B.pages_grow(c, 2), dict(slots=0, n=2), D.E_DESC),
-    (lambda c: B.pages_grow(c, 2), dict(page_size=0), D.E_DESC), (lambda c: B.pages_grow(c, 2), dict(aux_arg=-1), D.E_DESC),
+    (lambda c: B.pages_grow(c, 2), dict(page_size=0), D.E_DESC), (lambda c: B.pages_grow(c, 2), dict(pages=0), D.E_DESC), (lambda c: B.pages_grow(c, 2), dict(aux_arg=-1), D.E_DESC),
     (lambda c: B.pages_fork(c, 2), dict(pool_arg=-1), D.E_DESC), (lambda c: B.pages_fork(c, 2), dict(layers=3), D.E_OOB),
     (lambda c: B.pages_fork(c, 2), dict(page_bytes=24), D.E_DESC), (lambda c: B.pages_free(c, 2), dict(max_pages=5), D.E_OOB),
     (lambda c: B.pages_compact(c), dict(n=1), D.E_DESC), (lambda c: B.pages_compact(c), dict(pool_arg=0), D.E_UNSUPPORTED)])
