@@ -297,14 +297,20 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const __grid_constant__ K
       const uint32_t y = (x ^ (x >> 4)) & 0x00f000f0u;
       x ^= y ^ (y << 4);
     }
+    // Two bytes at a time: 1024 + lo + 16 hi, less 1024 + 16 hi is lo, and a sixteenth of that less 64 is hi, in fp16 and exact.
     uint32_t out[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t par = e < 2 ? p0[i] : p1[i];
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t par = e ? p1[i] : p0[i], x2 = __byte_perm(x, 0x64646464u, e ? 0x4342 : 0x4140), y = x2 & 0xfff0fff0u;
+      uint32_t lo, hi;
+      asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(x2), "r"(y));
+      asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(hi) : "r"(y), "r"(0x2c002c00u), "r"(0xd400d400u));
       const float s = lo_f32<F16>(par), mn = hi_f32<F16>(par);
-      const float c0 = __uint_as_float(((x >> (8 * e)) & 15u) | 0x4b000000u) - 8388608.f;
-      const float c1 = __uint_as_float(((x >> (8 * e + 4)) & 15u) | 0x4b000000u) - 8388608.f;
-      out[e] = pack_16x2<F16>(__fmaf_rn(s, c0, mn), __fmaf_rn(s, c1, mn));
+      const float2 s2 = make_float2(s, s), mn2 = make_float2(mn, mn);
+      const float2 a = __ffma2_rn(s2, make_float2(lo_f32<true>(lo), lo_f32<true>(hi)), mn2);
+      const float2 b = __ffma2_rn(s2, make_float2(hi_f32<true>(lo), hi_f32<true>(hi)), mn2);
+      out[2 * e] = pack_16x2<F16>(a.x, a.y);
+      out[2 * e + 1] = pack_16x2<F16>(b.x, b.y);
     }
     if (h >= g.hkv) continue;
     *reinterpret_cast<uint2 *>(dst + h * step_h + me.d0) = make_uint2(out[0], out[1]);
