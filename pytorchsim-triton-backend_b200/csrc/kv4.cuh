@@ -9,7 +9,7 @@
 // codes becomes two fp16 operands by half a byte permute (0x64 above the byte: 1024 + lo + 16 hi), one mask-and-or
 // (1032 + 16 hi), one subtraction (lo - 8) and one fused multiply-add (hi - 8), two of them on the FMA pipe; bf16, with 7 bits
 // of mantissa, takes a shift more per pair, all on the half-rate ALU pipe, which bounded that form (63 % busy, 467 warp
-// instructions per 16 keys, 166 us at 4 slots of up to 131072 keys).  bf16 queries fit fp16 after division by their row's power of
+// instructions per 16 keys, 166 us of kernel at 4 slots of up to 131072 keys; this one 312 and 111 us).  bf16 queries fit fp16 after division by their row's power of
 // two; the weights' V scales by a power of two that follows the largest scale seen.  The operands are centred because a
 // constant offset costs the sums their low bits: with 128 + c for V, 10^5 keys ended 2.4e-2 off (the tensor core truncates).
 //
@@ -20,7 +20,9 @@
 // without bank conflicts give words whose nibbles are the fragments.
 //
 // Bound: HBM, (D + 8 D / group) bytes per key and KV head (144 at D 128, group 64: 3.5 times fewer than bf16), and before
-// it the issue slots of the unpacking.  Work is one list of 64-key tiles over (slot, KV head), cut into equal contiguous
+// it the issue slots of the unpacking (60 % busy with three warps per scheduler, ALU 47 %; a fourth warp, at 128 registers,
+// changed nothing).  Both kernels: 64 slots of up to 8191 keys 65 us, 3.7 TB/s of cache; 4 slots of up to 131072 keys 118 us,
+// 4.1 TB/s, 0.64 of the measured copy bandwidth.  Work is one list of 64-key tiles over (slot, KV head), cut into equal contiguous
 // ranges, one per warp: a warp streams its tiles by bulk copies through a ring of its own (no barrier between warps) and keeps
 // the online softmax in registers.  Lengths are read on the device, so any raggedness is balanced to a tile.  A range that
 // holds only part of an item leaves (m, l, O) in the workspace and a second kernel (a programmatic dependent) merges the parts
@@ -188,6 +190,8 @@ __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], const floa
 
 // One (token, head) per D / 4 lanes, eight values a lane, `HS` steps of 128 / D heads a warp: their loads are issued before the
 // token's place is looked up, so a warp waits for the two once.  Extremes are packed 16-bit minima of x and -x, one shuffle a step.
+// HBM is the floor (K and V read, D + 8 D / group bytes written per head: 16 us at 24062 tokens of 8 heads of 128), the issue slots
+// bound it: 230 warp instructions per (token, head), 73 % busy, 59 us; 135 us with divisions and one head a warp.
 template <int D, int NG, bool F16, int HS>
 __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ Kv4Args g, uint8_t *pool) {
   constexpr int kLanes = D / 4, kHeads = 32 / kLanes, kGroup = D / NG;
@@ -258,6 +262,8 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ 
   }
 }
 
+// The reverse, the same lanes and steps: 120 warp instructions per (token, head), 31 us where the bytes take 16; 78 us with one
+// head a warp.
 template <int D, int NG, bool F16, int HS>
 __global__ void __launch_bounds__(256) kv4_load_kernel(const __grid_constant__ Kv4Args g) {
   constexpr int kLanes = D / 4, kHeads = 32 / kLanes, kGroup = D / NG;
@@ -864,8 +870,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kerne
 // Merges the parts of an item that several workers hold, in key order; zeros for an empty slot.  grid (slots x items, row
 // blocks of 128 / D rows), D / 4 lanes of four columns a row.  Each of the four warps goes over a quarter of the parts, D / 4 at a
 // time: lane j fetches part j's (m, l) of the row, the maximum and the weights are shuffles, and the columns' loads of eight
-// parts are in flight together; the quarters meet in shared memory.  (A thread per column that walks the parts one by one costs two dependent loads a part: 116 us in the
-// place of 20 for 16 rows of 33 slots cut into 40 parts.)
+// parts are in flight together; the quarters meet in shared memory.  (A thread per column that walked the parts one by one, two
+// dependent loads a part, made 116 us of a call that now takes 19: 33 slots, 16 rows a KV head, about 40 parts an item.)
 template <int D, bool F16>
 __global__ void __launch_bounds__(128) kv4_merge_kernel(const __grid_constant__ Kv4Args g) {
   constexpr int kLanes = D / 4, kRows = 32 / kLanes;

@@ -771,6 +771,36 @@ def test_captured_graphs_replay_on_two_streams():
     near(ob, *wb, torch.bfloat16)
 
 
+def test_a_captured_decode_step_grows_its_slots():
+    """Grow, store and attend as one replayed graph: the capture's own first run is a step, then each replay is one."""
+    slots, hq, hkv = 4, 8, 2
+    c = B.kv4_cache(slots=slots, max_pages=4, pages=16, hkv=hkv, dim=128, page_size=16, group=64)
+    state = {"ids": ints([0, 1, 2, 3]), "one": ints([1] * 4), "table": ints([[-1] * 4] * 4), "lens": ints([0] * 4), "refs": ints([0] * 16),
+             "pool": torch.zeros(c.pool_bytes, dtype=torch.uint8, device="cuda"), "cu": ints(range(5)),
+             "qkv": torch.zeros(slots, hq + 2 * hkv, 128, dtype=torch.bfloat16, device="cuda"),
+             "o": torch.zeros(slots, hq, 128, dtype=torch.bfloat16, device="cuda")}
+    g = Graph("cuda:0")
+    for name, t in state.items():
+        g.bind(name, t)
+    g.add("grow", D.to_bytes(B.pages_grow(c, slots)), ["ids", "one", "table", "lens", "refs"])
+    g.add("store", D.to_bytes(B.kv4_store(c, slots, fused_hq=hq)), ["qkv", "cu", "lens", "table", "pool"])
+    g.add("attend", D.to_bytes(B.attention_kv4(c, hq, fused=True)), ["qkv", "lens", "table", "pool", "o"])
+    past, r = [], gen(90)
+    for step in range(40):
+        state["qkv"].copy_(torch.randn(slots, hq + 2 * hkv, 128, generator=r).to(torch.bfloat16))
+        past.append(state["qkv"].clone())
+        if step == 0:
+            g.capture()
+        else:
+            g.run()
+        if step in (0, 15, 16, 39):
+            native.sync(torch.cuda.current_stream().cuda_stream)
+            rows = torch.stack(past, 1).flatten(0, 1)          # slot by slot
+            q, k, v = (x.contiguous() for x in rows.split([hq, hkv, hkv], 1))
+            near(state["o"], *cache_attention(past[-1][:, :hq], k, v, [step + 1] * slots, 64, 1 / math.sqrt(128)), torch.bfloat16)
+    assert state["lens"].tolist() == [40] * 4 and int((state["refs"] > 0).sum()) == 12
+
+
 def test_launches_on_two_streams_do_not_share_a_workspace():
     def case(seed, n):
         c, table, pool = cache_case([n], 128, 16, 64, 1, "bfloat16", seed)
