@@ -27,13 +27,13 @@ def attention_packed(q, k, v, cuq, cuk, scale, o):
 
 
 def quantise(x, group):
-    """(codes int64 [..., D], scale, minimum [..., D / group]) of x, in the arithmetic of its definition: fp32 quotients."""
+    """(codes int64 [..., D], scale, minimum [..., D / group]) of x, in the arithmetic of its definition: fp32 quotients of halves."""
     g = x.unflatten(-1, (-1, group)).float()
     mn, mx = g.amin(-1), g.amax(-1)
     scale = ((mx * 0.5 - mn * 0.5) / 7.5).to(x.dtype)
     bad = ~torch.isfinite(mx * 0.5 - mn * 0.5)
-    step = scale.float()[..., None]
-    code = torch.where(step > 0, torch.round((g - mn[..., None]) / step), 0.0).clamp(0, 15)
+    half = scale.float()[..., None] * 0.5          # halves throughout: exact, and the largest range does not overflow
+    code = torch.where(half > 0, torch.round((g * 0.5 - mn[..., None] * 0.5) / half), 0.0).clamp(0, 15)
     code = torch.where(bad[..., None], 0.0, code)
     nan = float("nan")
     return (code.to(torch.int64).flatten(-2), torch.where(bad, nan, scale.float()).to(x.dtype),

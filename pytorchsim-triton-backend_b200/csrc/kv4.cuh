@@ -127,11 +127,17 @@ __device__ __forceinline__ uint32_t min_16x2(uint32_t a, uint32_t b) {
   else asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
-// (minimum, -maximum) of two words' four values, as a pair.
 template <bool F16>
-__device__ __forceinline__ uint32_t extremes(uint32_t w0, uint32_t w1) {
-  const uint32_t lo = min_16x2<F16>(w0, w1), hi = min_16x2<F16>(w0 ^ 0x80008000u, w1 ^ 0x80008000u);
-  return min_16x2<F16>(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
+__device__ __forceinline__ uint32_t max_16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (F16) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// (minimum, -maximum), as a pair, of two minima and two maxima.
+template <bool F16>
+__device__ __forceinline__ uint32_t extremes(uint32_t lo, uint32_t hi) {
+  return min_16x2<F16>(__byte_perm(lo, hi, 0x5410) ^ 0x80000000u, __byte_perm(lo, hi, 0x7632) ^ 0x80000000u);
 }
 
 // half / 7.5 correctly rounded: the quotient by the rounded reciprocal, corrected by its exact remainder (Markstein's
@@ -142,50 +148,43 @@ __device__ __forceinline__ float over_seven_and_a_half(float half) {
   return fmaf(fmaf(-7.5f, q, half), r, q);
 }
 
-// Eight values (two runs of four, a scale and a minimum for each) to codes, nibble e the e-th value.  rint of the fp32
-// quotient y / step, y = x - mn, is the code.  The quotient by the reciprocal is within 2^-18 of it, so the two round alike unless it
-// lies that near to a half, n + 1/2 say, as every 400th value of a bf16 grid does exactly; then y is compared with
-// (n + 1/2) step, which fp32 holds exactly (11 bits times 5), and a tie goes to the even code.  (Only a quotient of 1/2 + 2^-25 would
-// be rounded to the tie and is not one; it takes a y of 24 bits.)  A float plus 1.5 * 2^23 is rounded to an integer in its low bits.
+// Eight values (two runs of four, a scale and a minimum for each) to codes, nibble e the e-th value: rint of the fp32 quotient
+// y / step, y = x - mn.  The quotient by the approximate reciprocal, corrected by its exact remainder, is within 2^-43 of y / step
+// before its rounding, and no y / step (24 bits by at most 11) lies on or within 2^-35 of the middle of two floats: it
+// is the rounded quotient, ties of codes (every 400th value of a bf16 grid) included.  A float plus 1.5 * 2^23 is rounded to an
+// integer in its low bits; the sums' upper halves hold what is left of that constant and are dropped.
 template <bool F16>
 __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], const float (&step)[2], const float (&mn)[2]) {
-  // Steps from kTiny on are rounded by at most 2^-9 of themselves: no quotient passes 15.5, and the reciprocal is a normal number.
-  constexpr float kMagic = 12582912.f, kTiny = F16 ? 6.103515625e-5f : 1e-30f;
-  uint32_t word = 0;
-  float y[8], d[8], n[8], r[2], odd = 0.f;
+  // Steps from kTiny on are rounded by at most 2^-9 of themselves: no quotient passes 15.5, remainders are exact and the
+  // reciprocal is a normal number; up to kHuge y does not overflow.
+  constexpr float kMagic = 12582912.f, kTiny = F16 ? 6.103515625e-5f : 1e-30f, kHuge = 2e37f;
+  uint32_t half[2] = {0, 0};
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r[k]) : "f"(step[k]));
-    if (step[k] < kTiny) r[k] = 0.f;
-  }
+    const float2 m2 = make_float2(-mn[k], -mn[k]), s2 = make_float2(-step[k], -step[k]);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(step[k]));
+    const float2 r2 = make_float2(r, r);
 #pragma unroll
-  for (int e = 0; e < 8; e += 2) {
-    const float m = -mn[e >> 2], k = r[e >> 2];
-    const float2 magic = make_float2(kMagic, kMagic), y2 = __fadd2_rn(make_float2(lo_f32<F16>(w[e >> 1]), hi_f32<F16>(w[e >> 1])), make_float2(m, m));
-    const float2 t2 = __ffma2_rn(y2, make_float2(k, k), magic), n2 = __fadd2_rn(t2, make_float2(-kMagic, -kMagic));
-    const float2 d2 = __ffma2_rn(y2, make_float2(k, k), make_float2(-n2.x, -n2.y));
-    y[e] = y2.x, y[e + 1] = y2.y, n[e] = n2.x, n[e + 1] = n2.y, d[e] = d2.x, d[e + 1] = d2.y;
-    odd = fmaxf(odd, fmaxf(fabsf(d2.x), fabsf(d2.y)));
-    word += (__float_as_uint(t2.x) << (4 * e)) + (__float_as_uint(t2.y) << (4 * e + 4));
-  }
-  constexpr uint32_t base = 0x4b400000u;
-  word -= base + (base << 4) + (base << 8) + (base << 12) + (base << 16) + (base << 20) + (base << 24) + (base << 28);
-  // Also one value after the other: a step too small for its reciprocal, and a run without one (a constant, or no number).
-  if (odd > 0.49999f || step[0] < kTiny || step[1] < kTiny) {
-    word = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float s = step[e >> 2];
-      float c = n[e];
-      if (fabsf(d[e]) > 0.49999f) {
-        const float below = d[e] > 0.f ? n[e] : n[e] - 1.f, tie = (below + 0.5f) * s;
-        c = y[e] > tie || (y[e] == tie && (int(below) & 1)) ? below + 1.f : below;
-      }
-      if (s < kTiny) c = s > 0.f ? rintf(__fdiv_rn(y[e], s)) : 0.f;
-      word |= uint32_t(fminf(fmaxf(c, 0.f), 15.f)) << (4 * e);
+    for (int e = 0; e < 4; e += 2) {
+      const uint32_t x = w[2 * k + e / 2];
+      const float2 y = __fadd2_rn(make_float2(lo_f32<F16>(x), hi_f32<F16>(x)), m2), q0 = __fmul2_rn(y, r2);
+      const float2 q = __ffma2_rn(__ffma2_rn(s2, q0, y), r2, q0), t = __fadd2_rn(q, make_float2(kMagic, kMagic));
+      half[k] += (__float_as_uint(t.x) << (4 * e)) + (__float_as_uint(t.y) << (4 * e + 4));
     }
+    // A step too small for its reciprocal or a range too large for y: halves, which fp32 holds exactly, and the division.
+    if ((step[k] < kTiny && step[k] > 0.f) || (!F16 && step[k] > kHuge)) {
+      half[k] = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t x = w[2 * k + e / 2];
+        const float y = (e & 1 ? hi_f32<F16>(x) : lo_f32<F16>(x)) * 0.5f - mn[k] * 0.5f;
+        half[k] |= uint32_t(fminf(rintf(__fdiv_rn(y, step[k] * 0.5f)), 15.f)) << (4 * e);
+      }
+    }
+    if (step[k] == 0.f) half[k] = 0;                                    // a constant, or no number
   }
-  return word;
+  return __byte_perm(half[0], half[1], 0x5410);
 }
 
 // One (token, head) per D / 4 lanes, eight values a lane, `HS` steps of 128 / D heads a warp: their loads are issued before the
@@ -227,9 +226,10 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ 
   for (int i = 0; i < HS; ++i) {
     const int h = h0 + i * kHeads;
     // (minimum, -maximum) of the lane's two runs of four; one group but for V in groups of 32.
-    uint32_t m0 = extremes<F16>(w[i][0], w[i][1]), m1 = extremes<F16>(w[i][2], w[i][3]);
-    const uint32_t both = min_16x2<F16>(m0, m1);
-    if (kGroup > 32 || !me.is_v) m0 = m1 = both;
+    const uint32_t lo0 = min_16x2<F16>(w[i][0], w[i][1]), lo1 = min_16x2<F16>(w[i][2], w[i][3]);
+    const uint32_t hi0 = max_16x2<F16>(w[i][0], w[i][1]), hi1 = max_16x2<F16>(w[i][2], w[i][3]);
+    uint32_t m0 = extremes<F16>(min_16x2<F16>(lo0, lo1), max_16x2<F16>(hi0, hi1)), m1 = m0;
+    if (kGroup == 32 && me.is_v) m0 = extremes<F16>(lo0, hi0), m1 = extremes<F16>(lo1, hi1);
     // Lanes of a group: group / 8 consecutive ones (V in groups of 32: the eight lanes of its 64 values, by run).
 #pragma unroll
     for (int s = 1; s < (kGroup > 64 ? 16 : 8); s *= 2) {

@@ -351,6 +351,34 @@ def test_store_of_many_tokens_is_the_store_of_few(dim, group, hkv, dtype, page):
         assert bool(((got.double() - want).abs() <= lim).all())
 
 
+@pytest.mark.parametrize("dim,group", [(128, 64), (128, 32), (64, 64)])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_codes_at_ties_and_at_the_ends_of_the_range(dim, group, dtype):
+    """Values halfway between codes, exponents far apart, the smallest and the largest groups: each code is the defined one, so
+    that what is read back is scale * code + minimum, one fp32 operation rounded once to the type."""
+    t, r, n = DT[dtype], gen(91), 600
+    low, high = (-126, 125) if dtype == "bfloat16" else (-14, 11)
+    grid = torch.randint(0, 31, (n, 2, dim), generator=r).double() * 0.5
+    grid.unflatten(-1, (-1, group))[..., 0], grid.unflatten(-1, (-1, group))[..., 1] = 0, 15   # the step is a power of two, ties abound
+    grid = grid * 2.0 ** torch.randint(low + 1, high - 4, (n, 2, 1), generator=r).double()
+    sign = torch.randint(0, 2, (n, 2, dim), generator=r).double() * 2 - 1
+    apart = sign * 2.0 ** (torch.rand(n, 2, dim, generator=r).double() * 30 - 20).clamp(low, high)
+    top = (torch.rand(n, 2, dim, generator=r).double() * 2 - 1) * torch.finfo(t).max
+    tiny = torch.randint(-400, 400, (n, 2, dim), generator=r).double() * torch.finfo(t).smallest_normal * torch.finfo(t).eps
+    edge = torch.rand(n, 2, dim, generator=r).double() * (15 if dtype == "bfloat16" else 1) * (1e-30 if dtype == "bfloat16" else 9e-4)
+    x = torch.cat([grid, apart, top, tiny, edge]).to(t)
+    c, table, pool = cache_case([5 * n], dim, 32, group, 2, dtype, 3)
+    books = [ints([0, 5 * n]), ints([5 * n]), ints(table), pool]
+    k, v = x.cuda(), x.flip(0).contiguous().cuda()
+    launch(B.kv4_store(c, 5 * n), [k, v] + books)
+    kb, vb = torch.zeros_like(k), torch.zeros_like(v)
+    launch(B.kv4_load(c, 5 * n), books + [kb, vb])
+    for got, put in ((kb.cpu(), k.cpu()), (vb.cpu(), v.cpu())):
+        code, scale, mn = S.quantise(put, group)
+        want = code.unflatten(-1, (-1, group)).double() * scale.double()[..., None] + mn.double()[..., None]
+        assert torch.equal(got, want.flatten(-2).float().to(t))
+
+
 def test_a_cache_past_four_gigabytes():
     """Pages whose records lie past 2^32 bytes: written, read, attended to, and moved."""
     pages, lens = 300000, [33, 20]
