@@ -195,9 +195,8 @@ template <int D, int NG, bool F16, int HS>
 __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ Kv4Args g, uint8_t *pool) {
   constexpr int kLanes = D / 4, kHeads = 32 / kLanes, kGroup = D / NG;
   const int lane = threadIdx.x & 31;
-  const uint32_t per_token = uint32_t(g.hkv + kHeads * HS - 1) / uint32_t(kHeads * HS);   // warps of a token
-  const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5), t = unit / per_token;
-  const int h0 = int(unit - t * per_token) * (kHeads * HS) + lane / kLanes;
+  const uint32_t t = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int h0 = int(blockIdx.y) * (kHeads * HS) + lane / kLanes;
   pdl_enter();
   if (t >= uint32_t(g.tokens)) return;
   const Kv4Lane<D, NG> me(lane);
@@ -268,9 +267,8 @@ template <int D, int NG, bool F16, int HS>
 __global__ void __launch_bounds__(256) kv4_load_kernel(const __grid_constant__ Kv4Args g) {
   constexpr int kLanes = D / 4, kHeads = 32 / kLanes, kGroup = D / NG;
   const int lane = threadIdx.x & 31;
-  const uint32_t per_token = uint32_t(g.hkv + kHeads * HS - 1) / uint32_t(kHeads * HS);
-  const uint32_t unit = blockIdx.x * 8 + (threadIdx.x >> 5), t = unit / per_token;
-  const int h0 = int(unit - t * per_token) * (kHeads * HS) + lane / kLanes;
+  const uint32_t t = blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int h0 = int(blockIdx.y) * (kHeads * HS) + lane / kLanes;
   pdl_enter();
   if (t >= uint32_t(g.tokens)) return;
   int64_t pos = 0;
@@ -975,7 +973,7 @@ static int run_kv4(const ptsim_desc &d, Kv4Args &g, uint8_t *pool, const LaunchC
   constexpr int kHeads = 128 / D;
   const int64_t four = g.tokens * ceil_div(g.hkv, 4 * kHeads), one = g.tokens * ceil_div(g.hkv, kHeads);
   const bool many = four >= int64_t(c.sm_count) * 32;
-  const dim3 grid(unsigned(ceil_div(many ? four : one, 8)));
+  const dim3 grid(unsigned(ceil_div(g.tokens, 8)), unsigned(ceil_div(g.hkv, many ? 4 * kHeads : kHeads)));
   if (d.kind == PTSIM_KIND_KV4_STORE)
     PTSIM_CUDA(launch_pdl(many ? kv4_store_kernel<D, NG, F16, 4> : kv4_store_kernel<D, NG, F16, 1>, grid, dim3(256), 0, c.stream, g, pool));
   else
