@@ -152,39 +152,47 @@ __device__ __forceinline__ float over_seven_and_a_half(float half) {
 // y / step, y = x - mn.  The quotient by the approximate reciprocal, corrected by its exact remainder, is within 2^-43 of y / step
 // before its rounding, and no y / step (24 bits by at most 11) lies on or within 2^-35 of the middle of two floats: it
 // is the rounded quotient, ties of codes (every 400th value of a bf16 grid) included.  A float plus 1.5 * 2^23 is rounded to an
-// integer in its low bits; the sums' upper halves hold what is left of that constant and are dropped.
+// integer in its low byte; of the eight bytes `even` takes the low nibbles of the result, `odd` the high ones.
 template <bool F16>
-__device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], const float (&step)[2], const float (&mn)[2]) {
+__device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], const float (&step)[2], const float (&mn)[2], uint32_t even, uint32_t odd) {
   // Steps from kTiny on are rounded by at most 2^-9 of themselves: no quotient passes 15.5, remainders are exact and the
   // reciprocal is a normal number; up to kHuge y does not overflow.
   constexpr float kMagic = 12582912.f, kTiny = F16 ? 6.103515625e-5f : 1e-30f, kHuge = 2e37f;
-  uint32_t half[2] = {0, 0};
+  uint32_t run[2];                     // the codes of four values, one a byte
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const float2 m2 = make_float2(-mn[k], -mn[k]), s2 = make_float2(-step[k], -step[k]);
     float r;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(step[k]));
     const float2 r2 = make_float2(r, r);
+    uint32_t pair[2];
 #pragma unroll
-    for (int e = 0; e < 4; e += 2) {
-      const uint32_t x = w[2 * k + e / 2];
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t x = w[2 * k + e];
       const float2 y = __fadd2_rn(make_float2(lo_f32<F16>(x), hi_f32<F16>(x)), m2), q0 = __fmul2_rn(y, r2);
       const float2 q = __ffma2_rn(__ffma2_rn(s2, q0, y), r2, q0), t = __fadd2_rn(q, make_float2(kMagic, kMagic));
-      half[k] += (__float_as_uint(t.x) << (4 * e)) + (__float_as_uint(t.y) << (4 * e + 4));
+      pair[e] = __byte_perm(__float_as_uint(t.x), __float_as_uint(t.y), 0x0040);
     }
-    // A step too small for its reciprocal or a range too large for y: halves, which fp32 holds exactly, and the division.
-    if ((step[k] < kTiny && step[k] > 0.f) || (!F16 && step[k] > kHuge)) {
-      half[k] = 0;
+    run[k] = __byte_perm(pair[0], pair[1], 0x5410);
+  }
+  // A step too small for its reciprocal or a range too large for y: halves, which fp32 holds exactly, and the division.  No step (a
+  // constant, or no number): code 0.
+  const auto rare = [](float s) { return s < kTiny || (!F16 && s > kHuge); };
+  if (rare(step[0]) || rare(step[1])) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (!rare(step[k])) continue;
+      run[k] = 0;
+      if (step[k] == 0.f) continue;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const uint32_t x = w[2 * k + e / 2];
         const float y = (e & 1 ? hi_f32<F16>(x) : lo_f32<F16>(x)) * 0.5f - mn[k] * 0.5f;
-        half[k] |= uint32_t(fminf(rintf(__fdiv_rn(y, step[k] * 0.5f)), 15.f)) << (4 * e);
+        run[k] |= uint32_t(fminf(rintf(__fdiv_rn(y, step[k] * 0.5f)), 15.f)) << (8 * e);
       }
     }
-    if (step[k] == 0.f) half[k] = 0;                                    // a constant, or no number
   }
-  return __byte_perm(half[0], half[1], 0x5410);
+  return __byte_perm(run[0], run[1], even) + 16 * __byte_perm(run[0], run[1], odd);
 }
 
 // One (token, head) per D / 4 lanes, eight values a lane, `HS` steps of 128 / D heads a warp: their loads are issued before the
@@ -221,6 +229,7 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ 
   int code_at, par_at;
   me.place(int(pos) & ((1 << g.page_log) - 1), g.page_log, &code_at, &par_at);
   uint8_t *rec = pool + int64_t(page) * g.hkv * g.record;
+  const uint32_t even = me.is_v ? 0x6420 : 0x5140, odd = me.is_v ? 0x7531 : 0x7362;   // K: value d in nibble d / 2 + 4 (d % 2)
 #pragma unroll
   for (int i = 0; i < HS; ++i) {
     const int h = h0 + i * kHeads;
@@ -247,11 +256,7 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ 
       par[r] = fine ? pack_16x2<F16>(over_seven_and_a_half(half), mn[r]) : (F16 ? 0x7e007e00u : 0x7fc07fc0u);   // the minimum is exact
       step[r] = fine ? lo_f32<F16>(par[r]) : 0.f;                         // a group that is no number: codes 0
     }
-    uint32_t word = quantise8<F16>(w[i], step, mn);
-    if (!me.is_v) {                                                       // K: value d in nibble d / 2 + 4 (d % 2)
-      const uint32_t x = (word ^ (word >> 4)) & 0x00f000f0u;
-      word = __byte_perm(word ^ x ^ (x << 4), 0, 0x3120);
-    }
+    const uint32_t word = quantise8<F16>(w[i], step, mn, even, odd);
     if (h >= g.hkv) continue;
     uint8_t *to = rec + h * g.record;
     *reinterpret_cast<uint32_t *>(to + code_at) = word;
@@ -290,31 +295,28 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const __grid_constant__ K
     p0[i] = *reinterpret_cast<const uint32_t *>(at + par_at + 4 * (me.d0 / kGroup));
     p1[i] = kGroup > 32 ? p0[i] : *reinterpret_cast<const uint32_t *>(at + par_at + 4 * (me.d1 / kGroup));
   }
+  // Bytes of values 0 - 3 and 4 - 7: K keeps value d in nibble d / 2 + 4 (d % 2), so low nibbles are one pair, V value e in nibble e.
+  const uint32_t bytes0 = me.is_v ? 0x4140 : 0x4240, bytes1 = me.is_v ? 0x4342 : 0x4341;
+  const uint32_t pair0 = me.is_v ? 0x5410 : 0x3210, pair1 = me.is_v ? 0x7632 : 0x7654;
   uint16_t *dst = me.is_v ? g.b + t * g.b_row : g.a + t * g.a_row;
   const int64_t step_h = me.is_v ? g.b_head : g.a_head;
 #pragma unroll
   for (int i = 0; i < HS; ++i) {
     const int h = h0 + i * kHeads;
-    uint32_t x = word[i];
-    if (!me.is_v) {                                           // K: nibble d / 2 + 4 (d % 2) to nibble d
-      x = __byte_perm(x, 0, 0x3120);
-      const uint32_t y = (x ^ (x >> 4)) & 0x00f000f0u;
-      x ^= y ^ (y << 4);
-    }
     // Two bytes at a time: 1024 + lo + 16 hi, less 1024 + 16 hi is lo, and a sixteenth of that less 64 is hi, in fp16 and exact.
     uint32_t out[4];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const uint32_t par = e ? p1[i] : p0[i], x2 = __byte_perm(x, 0x64646464u, e ? 0x4342 : 0x4140), y = x2 & 0xfff0fff0u;
+      const uint32_t par = e ? p1[i] : p0[i], x2 = __byte_perm(word[i], 0x64646464u, e ? bytes1 : bytes0), y = x2 & 0xfff0fff0u;
       uint32_t lo, hi;
       asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(x2), "r"(y));
       asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(hi) : "r"(y), "r"(0x2c002c00u), "r"(0xd400d400u));
       const float s = lo_f32<F16>(par), mn = hi_f32<F16>(par);
       const float2 s2 = make_float2(s, s), mn2 = make_float2(mn, mn);
-      const float2 a = __ffma2_rn(s2, make_float2(lo_f32<true>(lo), lo_f32<true>(hi)), mn2);
-      const float2 b = __ffma2_rn(s2, make_float2(hi_f32<true>(lo), hi_f32<true>(hi)), mn2);
-      out[2 * e] = pack_16x2<F16>(a.x, a.y);
-      out[2 * e + 1] = pack_16x2<F16>(b.x, b.y);
+      const float2 a = __ffma2_rn(s2, make_float2(lo_f32<true>(lo), hi_f32<true>(lo)), mn2);
+      const float2 b = __ffma2_rn(s2, make_float2(lo_f32<true>(hi), hi_f32<true>(hi)), mn2);
+      const uint32_t o0 = pack_16x2<F16>(a.x, a.y), o1 = pack_16x2<F16>(b.x, b.y);
+      out[2 * e] = __byte_perm(o0, o1, pair0), out[2 * e + 1] = __byte_perm(o0, o1, pair1);
     }
     if (h >= g.hkv) continue;
     *reinterpret_cast<uint2 *>(dst + h * step_h + me.d0) = make_uint2(out[0], out[1]);
@@ -971,13 +973,13 @@ static int run_kv4(const ptsim_desc &d, Kv4Args &g, uint8_t *pool, const LaunchC
   // A warp takes four steps of heads where that leaves every SM 32 warps or more, else one, so that a decode step's few tokens
   // spread.
   constexpr int kHeads = 128 / D;
-  const int64_t four = g.tokens * ceil_div(g.hkv, 4 * kHeads), one = g.tokens * ceil_div(g.hkv, kHeads);
+  const int64_t four = g.tokens * ceil_div(g.hkv, 8 * kHeads), one = g.tokens * ceil_div(g.hkv, kHeads);
   const bool many = four >= int64_t(c.sm_count) * 32;
-  const dim3 grid(unsigned(ceil_div(g.tokens, 8)), unsigned(ceil_div(g.hkv, many ? 4 * kHeads : kHeads)));
+  const dim3 grid(unsigned(ceil_div(g.tokens, 8)), unsigned(ceil_div(g.hkv, many ? 8 * kHeads : kHeads)));
   if (d.kind == PTSIM_KIND_KV4_STORE)
-    PTSIM_CUDA(launch_pdl(many ? kv4_store_kernel<D, NG, F16, 4> : kv4_store_kernel<D, NG, F16, 1>, grid, dim3(256), 0, c.stream, g, pool));
+    PTSIM_CUDA(launch_pdl(many ? kv4_store_kernel<D, NG, F16, 8> : kv4_store_kernel<D, NG, F16, 1>, grid, dim3(256), 0, c.stream, g, pool));
   else
-    PTSIM_CUDA(launch_pdl(many ? kv4_load_kernel<D, NG, F16, 4> : kv4_load_kernel<D, NG, F16, 1>, grid, dim3(256), 0, c.stream, g));
+    PTSIM_CUDA(launch_pdl(many ? kv4_load_kernel<D, NG, F16, 8> : kv4_load_kernel<D, NG, F16, 1>, grid, dim3(256), 0, c.stream, g));
   return PTSIM_OK;
 }
 
