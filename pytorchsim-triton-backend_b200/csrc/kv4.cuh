@@ -198,7 +198,8 @@ __device__ __forceinline__ uint32_t quantise8(const uint32_t (&w)[4], const floa
 // One (token, head) per D / 4 lanes, eight values a lane, `HS` steps of 128 / D heads a warp: their loads are issued before the
 // token's place is looked up, so a warp waits for the two once.  Extremes are packed 16-bit minima of x and -x, one shuffle a step.
 // HBM is the floor (K and V read, D + 8 D / group bytes written per head: 16 us at 24062 tokens of 8 heads of 128), the issue slots
-// bound it: 230 warp instructions per (token, head), 73 % busy, 59 us; 135 us with divisions and one head a warp.
+// bound it: 143 warp instructions per (token, head), 71 % busy, 39 us; 135 us with divisions and one head a warp, 43 with four.
+// The lookup is 150 of a warp's instructions, so a grid of tokens by heads, without a division, and many steps.
 template <int D, int NG, bool F16, int HS>
 __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ Kv4Args g, uint8_t *pool) {
   constexpr int kLanes = D / 4, kHeads = 32 / kLanes, kGroup = D / NG;
@@ -233,6 +234,7 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ 
 #pragma unroll
   for (int i = 0; i < HS; ++i) {
     const int h = h0 + i * kHeads;
+    if (h - lane / kLanes >= g.hkv) break;                                // the whole warp
     // (minimum, -maximum) of the lane's two runs of four; one group but for V in groups of 32.
     const uint32_t lo0 = min_16x2<F16>(w[i][0], w[i][1]), lo1 = min_16x2<F16>(w[i][2], w[i][3]);
     const uint32_t hi0 = max_16x2<F16>(w[i][0], w[i][1]), hi1 = max_16x2<F16>(w[i][2], w[i][3]);
@@ -266,8 +268,8 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ 
   }
 }
 
-// The reverse, the same lanes and steps: 120 warp instructions per (token, head), 31 us where the bytes take 16; 78 us with one
-// head a warp.
+// The reverse, the same lanes and steps: 86 warp instructions per (token, head), 25 us where the bytes take 16; 78 us with one
+// head a warp, 28 with four.
 template <int D, int NG, bool F16, int HS>
 __global__ void __launch_bounds__(256) kv4_load_kernel(const __grid_constant__ Kv4Args g) {
   constexpr int kLanes = D / 4, kHeads = 32 / kLanes, kGroup = D / NG;
@@ -303,6 +305,7 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const __grid_constant__ K
 #pragma unroll
   for (int i = 0; i < HS; ++i) {
     const int h = h0 + i * kHeads;
+    if (h - lane / kLanes >= g.hkv) break;                    // the whole warp
     // Two bytes at a time: 1024 + lo + 16 hi, less 1024 + 16 hi is lo, and a sixteenth of that less 64 is hi, in fp16 and exact.
     uint32_t out[4];
 #pragma unroll
@@ -970,11 +973,11 @@ template <int D, int NG, bool F16>
 static int run_kv4(const ptsim_desc &d, Kv4Args &g, uint8_t *pool, const LaunchCtx &c) {
   if (d.kind == PTSIM_KIND_ATTN_KV4)
     return d.p.kv4.hq / d.p.kv4.hkv <= 8 ? run_kv4_attn<D, NG, 1, F16>(g, c) : run_kv4_attn<D, NG, 2, F16>(g, c);
-  // A warp takes four steps of heads where that leaves every SM 32 warps or more, else one, so that a decode step's few tokens
-  // spread.
+  // A warp takes eight steps of heads where that leaves every SM 12 warps or more, else one, so that few tokens spread: 600 tokens of
+  // 8 heads of 128 are stored and loaded in 11 us with one step and 13 with eight, 1200 in 15 with either, 4500 in 28 and 22.
   constexpr int kHeads = 128 / D;
-  const int64_t four = g.tokens * ceil_div(g.hkv, 8 * kHeads), one = g.tokens * ceil_div(g.hkv, kHeads);
-  const bool many = four >= int64_t(c.sm_count) * 32;
+  const int64_t eight = g.tokens * ceil_div(g.hkv, 8 * kHeads), one = g.tokens * ceil_div(g.hkv, kHeads);
+  const bool many = eight >= int64_t(c.sm_count) * 12 && one > eight;
   const dim3 grid(unsigned(ceil_div(g.tokens, 8)), unsigned(ceil_div(g.hkv, many ? 8 * kHeads : kHeads)));
   if (d.kind == PTSIM_KIND_KV4_STORE)
     PTSIM_CUDA(launch_pdl(many ? kv4_store_kernel<D, NG, F16, 8> : kv4_store_kernel<D, NG, F16, 1>, grid, dim3(256), 0, c.stream, g, pool));

@@ -105,7 +105,8 @@ static int check_rows(const ptsim_desc &d, int arg, int64_t off, int64_t row, in
     return fail(PTSIM_E_DESC, "%s: offset %lld, strides %lld and %lld", what, (long long)off, (long long)row, (long long)head);
   if (off % 8 != 0 || row % 8 != 0 || head % 8 != 0)
     return fail(PTSIM_E_UNSUPPORTED, "%s: its offset and strides must be multiples of 8 elements", what);
-  if (rows > 0 && off + (rows - 1) * row + (heads - 1) * head + dim > d.arg_numel[arg])
+  const __int128 end = off + __int128(rows - 1) * row + __int128(heads - 1) * head + dim;   // 64 bits could wrap
+  if (rows > 0 && end > d.arg_numel[arg])
     return fail(PTSIM_E_OOB, "%s extends past its tensor", what);
   return PTSIM_OK;
 }

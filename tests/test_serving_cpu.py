@@ -77,6 +77,14 @@ def test_packed_attention_refusals(fields, code):
     assert _code(_with(B.attention_packed(10, 3, 8, 2), "pattn", **fields)) == code
 
 
+def test_row_strides_whose_product_passes_64_bits_are_refused():
+    n, row = (1 << 27) + 1, 1 << 37                                  # the last row starts at 2^64
+    assert _code(_with(B.attention_packed(10, 3, 8, 2), "pattn", q_tokens=n, q_row=row, o_row=row)) == D.E_OOB
+    assert _code(_with(B.attention_packed(10, 3, 8, 2), "pattn", k_tokens=n, k_row=row, v_row=row)) == D.E_OOB
+    for make in (B.kv4_store, B.kv4_load):
+        assert _code(_with(make(shape(), 7), "kv4", tokens=n, a_row=row, b_row=row)) == D.E_OOB
+
+
 @pytest.mark.parametrize("make", [lambda c: B.kv4_store(c, 7), lambda c: B.kv4_load(c, 7), lambda c: B.attention_kv4(c, 6)])
 @pytest.mark.parametrize("fields,code", [
     (dict(dim=32), D.E_UNSUPPORTED), (dict(group=16), D.E_UNSUPPORTED), (dict(page_size=8), D.E_UNSUPPORTED),
