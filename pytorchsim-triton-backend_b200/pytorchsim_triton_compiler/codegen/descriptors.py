@@ -18,8 +18,15 @@ KIND_NAME = {ELEMENTWISE: "elementwise", ROW_SOFTMAX: "row_softmax", ROW_RMSNORM
              QKNORM_ROPE: "qknorm_rope", GEMM: "gemm", ATTN_PREFILL: "attn_prefill", REDUCE_ALL: "reduce_all",
              ATTN_DECODE: "attn_decode", ROW_DIVSUM: "row_divsum", TOPK: "topk", SORT: "sort",
              GATHER_ROWS: "gather_rows", GROUPED_GEMM: "grouped_gemm", GATHER_SUM: "gather_sum",
-             INT_TABLE: "int_table", ROW_SUM: "row_sum", ATTN_PACKED: "attn_packed", KV4_STORE: "kv4_store",
-             KV4_LOAD: "kv4_load", ATTN_KV4: "attn_kv4", PAGES: "pages"}
+             INT_TABLE: "int_table", ROW_SUM: "row_sum"}
+# Kinds that no tile program lowers to: a program builds and launches them directly.
+SERVING_NAME = {ATTN_PACKED: "attn_packed", KV4_STORE: "kv4_store", KV4_LOAD: "kv4_load", ATTN_KV4: "attn_kv4", PAGES: "pages"}
+
+
+def kind_name(kind):
+    """The name of a descriptor kind, the kind itself where it has none."""
+    return KIND_NAME.get(kind, SERVING_NAME.get(kind, kind))
+
 
 # Element types (PTSIM_DT_*), keyed by kernel.json dtype names (contract/kernel_object.py NP_DTYPE keys).
 DTYPE_CODE = {"float32": 0, "bfloat16": 1, "float16": 2, "int32": 3, "int64": 4, "int16": 5, "int8": 6,
@@ -244,7 +251,7 @@ def describe_vprog(v):
 
 def describe(d):
     """A JSON-able summary of descriptor `d` (what kernel.json records next to the blob)."""
-    out = {"kind": KIND_NAME.get(d.kind, d.kind), "units": d.units, "unit_size": d.unit_size,
+    out = {"kind": kind_name(d.kind), "units": d.units, "unit_size": d.unit_size,
            "grid": list(d.grid), "workspace_bytes": d.workspace_bytes}
     if d.kind == ELEMENTWISE:
         e = d.p.ew

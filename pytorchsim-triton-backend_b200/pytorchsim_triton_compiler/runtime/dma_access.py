@@ -362,7 +362,7 @@ def write(runtime, manifest, desc, ranges, host=None):
     """Write dma_access/trace.json under `runtime` for the unit `ranges` ([(device, lo, hi)]) of a launch."""
     names = [a["name"] for a in manifest["args"]]
     dtypes = {a["name"]: a["dtype"] for a in manifest["args"]}
-    out = {"format": FORMAT, "kernel": manifest.get("name"), "kind": D.KIND_NAME.get(desc.kind, desc.kind),
+    out = {"format": FORMAT, "kernel": manifest.get("name"), "kind": D.kind_name(desc.kind),
            "ranges": [{"device": dev, "units": [lo, hi], "streams": streams(desc, lo, hi, names, dtypes, host)}
                       for dev, lo, hi in ranges]}
     path = os.path.join(runtime, DIR)

@@ -1,5 +1,7 @@
 """The serving operators without a GPU: their descriptors and refusals (ptsim_check), their access streams, and the
 64-bit oracle's own consistency (a token written into a record reads back as the values its codes stand for)."""
+import json
+
 import pytest
 import torch
 
@@ -42,7 +44,7 @@ def test_descriptors_validate_and_describe(name, desc):
     blob = D.to_bytes(desc)
     native.check(blob)
     assert native.units(blob) == 1
-    assert D.describe(D.from_bytes(blob))["kind"] == D.KIND_NAME[desc.kind]
+    assert D.describe(D.from_bytes(blob))["kind"] == D.SERVING_NAME[desc.kind]
     outs = RC.written_args(desc)
     names = [f"a{i}" for i in range(desc.nargs)]
     streams = dma_access.streams(desc, 0, 1, names)
@@ -203,3 +205,10 @@ def test_page_oracle_forks_frees_and_compacts():
     assert p.table[:2] == [[-1] * 3] * 2 and p.refs == [1, 1, 0, 0, 1, 0, 0, 0]
     p.compact()
     assert p.table[2] == [0, 1, 2] and p.refs == [1, 1, 1, 0, 0, 0, 0, 0]
+
+
+def test_the_command_line_names_the_serving_kinds(capsys):
+    from pytorchsim_triton_compiler import cli
+    cli.target()
+    got = json.loads(capsys.readouterr().out)["serving"]
+    assert got == ["attn_packed", "kv4_store", "kv4_load", "attn_kv4", "pages"] and D.kind_name(D.PAGES) == "pages" and D.kind_name(99) == 99
