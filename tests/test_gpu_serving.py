@@ -325,7 +325,8 @@ def test_store_writes_the_defined_bytes_and_load_reads_them(dim, page, group, hk
     assert bool((got[0] == 0xA5).all())                                       # the other layer
 
 
-@pytest.mark.parametrize("dim,group,hkv,dtype,page", [(128, 64, 5, "bfloat16", 16), (128, 32, 4, "float16", 64), (64, 32, 3, "bfloat16", 32)])
+@pytest.mark.parametrize("dim,group,hkv,dtype,page", [(128, 64, 5, "bfloat16", 16), (128, 32, 4, "float16", 64), (64, 32, 3, "bfloat16", 32),
+                                                        (128, 64, 9, "bfloat16", 16), (64, 64, 17, "float16", 128), (128, 128, 2, "bfloat16", 64)])
 def test_store_of_many_tokens_is_the_store_of_few(dim, group, hkv, dtype, page):
     """Several heads a warp (many tokens) and one (few) write the same bytes; the values are those of the definition."""
     lens = [4000, 1, 5100, 777]
