@@ -395,7 +395,7 @@ __device__ __forceinline__ int kv4_units(int tiles) { return tiles > 0 ? tiles +
 __device__ __forceinline__ uint32_t kv4_share(uint32_t total, int workers) { return (total + uint32_t(workers) - 1) / uint32_t(workers); }
 
 template <int D, int NG, int NT, bool F16>
-__global__ void __launch_bounds__(kKvWarps * 32, NT == 1 ? 3 : 2) kv4_attn_kernel(const __grid_constant__ Kv4Args g) {
+__global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && NG < 4 ? 3 : 2) kv4_attn_kernel(const __grid_constant__ Kv4Args g) {
   constexpr int kStage = kKvTile * (D + 8 * NG);            // bytes of a tile: two blocks of 32 keys or four of 16
   constexpr int kWordsK = D / 32, kWordsV = D / 64;         // words a lane takes of a K and of a V row
   constexpr int kGroup = D / NG;
@@ -948,8 +948,10 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const __grid_constant__ 
 }
 
 // Workers of a launch: one warp each, as many as are resident at once.
+// Warps of the attention: three CTAs an SM (168 registers a thread), two where 16 query heads or four groups of a head dimension take
+// more (64 slots of up to 8191 keys, groups of 32 at D 128: 83 us with two CTAs and 213 registers, 116 with three and spills).
 static int kv4_workers(const ptsim_kv4_params &p, int sm_count) {
-  return sm_count * (p.hq / p.hkv <= 8 ? 3 : 2) * kKvWarps;
+  return sm_count * (p.hq / p.hkv <= 8 && p.dim / p.group < 4 ? 3 : 2) * kKvWarps;
 }
 
 int64_t kv4_workspace(const ptsim_desc &d, int sm_count) {
