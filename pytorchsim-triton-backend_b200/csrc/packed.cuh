@@ -197,8 +197,10 @@ __global__ void __launch_bounds__(PackedShape<T>::kThreads, T == 2 ? 1 : 2) pack
       const int last = it.pos0 + (it.rows_b > 0 ? 128 + it.rows_b : it.rows_a);   // keys that the item's last row sees
       if (seq >= 0 && last > 0) {
         const int kvh = head / g.per;
-        sm100::mbar_arrive_expect_tx(q_full, it.rows_b > 0 ? 2 * kTile : kTile);
-        for (int t = 0; t < (it.rows_b > 0 ? 2 : 1); ++t)
+        // Only tiles that see a key: one that sees none has nothing to wait for before it stages its zeros over its Q.
+        const int t0 = it.pos0 + it.rows_a > 0 ? 0 : 1, t1 = it.rows_b > 0 ? 2 : 1;
+        sm100::mbar_arrive_expect_tx(q_full, (t1 - t0) * kTile);
+        for (int t = t0; t < t1; ++t)
           for (int c = 0; c < D / 64; ++c)
             sm100::tma_load_3d(sQ + t * kTile + c * kHalf, &g.tq, q_full, c * 64, it.q0 + t * 128, head);
         sm100::mbar_arrive_expect_tx(&k_full[0], kTile);
@@ -469,7 +471,8 @@ __global__ void __launch_bounds__(PackedShape<T>::kThreads, T == 2 ? 1 : 2) pack
       if (ok) {
         sm100::tc_fence_after();
         const float inv = pos < 0 ? 0.f : 1.0f / l;
-        // The warp's 32 rows, staged over Q (every product that reads this tile's is done), 16-byte units exchanged by row.
+        // The warp's 32 rows, staged over Q (every product that reads this tile's is done, or the tile was never loaded), 16-byte
+        // units exchanged by row.
         constexpr int kUnits = D / 8;
         uint8_t *mine = sQ + t * kTile + quarter * (kTile / 4);
         uint32_t v[D / 32][32];

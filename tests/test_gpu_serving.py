@@ -126,6 +126,27 @@ def test_packed_attention_of_long_sequences(ql, kl, dim, dtype):
     near(o, *dense(q, k, v, ql, kl, q0, k0, 1 / math.sqrt(dim)), DT[dtype])
 
 
+@pytest.mark.parametrize("dim,dtype,more,keys", [(128, "bfloat16", 700, 800), (128, "float16", 1152, 1024), (64, "bfloat16", 700, 4200)])
+def test_rows_without_keys_beside_a_tile_with_keys_are_zeros(dim, dtype, more, keys):
+    """`more` queries than keys: the first item with a key has none in its first tile.  The zeros of those rows take the place of Q
+    in shared memory, so Q of such a tile must not be on its way there."""
+    ql, kl = [keys + more + i % 3 for i in range(12)], [keys] * 12
+    assert all(128 <= (a - b) % 256 < 256 for a, b in zip(ql, kl))
+    q, k, v, q0, k0 = packed_case(ql, kl, 4, 1, dim, dtype, more)
+    desc = B.attention_packed(q0[-1], 12, 4, 1, dim, dtype=dtype, k_tokens=k0[-1])
+    first = None
+    for _ in range(20):
+        o = torch.full_like(q, 7.0)
+        launch(desc, [q, k, v, ints(q0), ints(k0), o])
+        for s in range(12):
+            assert not o[q0[s]:q0[s] + ql[s] - kl[s]].any()
+        first = o if first is None else first
+        assert torch.equal(o, first)
+    some = slice(q0[11], q0[12])
+    want, mag = dense(q[some], k[k0[11]:], v[k0[11]:], ql[11:], kl[11:], [0], [0], 1 / math.sqrt(dim))
+    near(first[some], want, mag, DT[dtype])
+
+
 def test_packed_attention_of_long_sequences_is_blind_to_keys_it_does_not_see():
     lens = [900, 1000, 800]
     q, k, v, q0, k0 = packed_case(lens, lens, 2, 1, 128, "bfloat16", 21)
