@@ -630,10 +630,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && NG < 4 ? 3 : 2) kv4_
     }
 
     for (int tile = first; tile < last; ++tile) {
-      if (!sm100::mbar_wait(&full[st], phase, wl)) {
-        ok = false;
-        break;
-      }
+      // The outcome is made the warp's: one lane must not leave a loop that others vote in.
+      if (!(ok = __all_sync(0xffffffffu, sm100::mbar_wait(&full[st], phase, wl)))) break;
       const int there = good[st];
 #pragma unroll 1
       for (int pass = 0; pass < kKvTile / kKvPass; ++pass) {

@@ -915,3 +915,22 @@ def test_stalled_stage_times_out_and_device_stays_usable(family):
     assert failed(stalled, ts) == D.E_TIMEOUT
     launch(desc, ts)
     near(o, *want, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dim,group,per,dtype", [(128, 64, 4, "bfloat16"), (64, 32, 12, "float16"), (128, 32, 9, "bfloat16")])
+def test_a_stalled_cache_tile_ends_its_own_part_only(dim, group, per, dtype):
+    """The warp whose first tile never lands gives up as a whole: the slots that it holds nothing of are computed."""
+    lens = [64] + [300] * 11
+    c, table, pool = cache_case(lens, dim, 16, group, 1, dtype, 84)
+    k, v = rows_of(sum(lens), c, 85)
+    q = torch.randn(12, per, dim, generator=gen(86)).to(DT[dtype]).cuda()
+    o, books = torch.full_like(q, 7.0), [ints(lens), ints(table), pool]
+    launch(B.kv4_store(c, sum(lens)), [k, v, ints(starts(lens))] + books)
+    stalled = B.attention_kv4(c, per)
+    stalled.flags |= D.FLAG_TEST_STALL
+    assert failed(stalled, [q] + books + [o]) == D.E_TIMEOUT
+    want, mag = cache_attention(q, k, v, lens, group, 1 / math.sqrt(dim))
+    near(o[1:], want[1:], mag[1:], DT[dtype])
+    assert bool((o[0] == 7).all())
+    launch(B.attention_kv4(c, per), [q] + books + [o])
+    near(o, want, mag, DT[dtype])
