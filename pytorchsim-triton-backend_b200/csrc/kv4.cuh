@@ -9,8 +9,8 @@
 // codes becomes two fp16 operands by half a byte permute (0x64 above the byte: 1024 + lo + 16 hi), one mask-and-or
 // (1032 + 16 hi), one subtraction (lo - 8) and one fused multiply-add (hi - 8), two of them on the FMA pipe; bf16, with 7 bits
 // of mantissa, takes a shift more per pair, all on the half-rate ALU pipe, which bounded that form (63 % busy, 467 warp
-// instructions per 16 keys, 166 us of kernel at 4 slots of up to 131072 keys; this one 312 and 111 us).  bf16 queries fit fp16 after division by their row's power of
-// two; the weights' V scales by a power of two that follows the largest scale seen.  The operands are centred because a
+// instructions per 16 keys, 166 us of kernel at 4 slots of up to 131072 keys; this one 312 and 111 us).  Queries fit fp16 after division
+// by their row's power of two; the weights' V scales, of bf16 caches, by a power of two that follows the largest scale seen.  The operands are centred because a
 // constant offset costs the sums their low bits: with 128 + c for V, 10^5 keys ended 2.4e-2 off (the tensor core truncates).
 //
 // The products have K and V as the 16-row operand: S^T = K q^T, O^T = V^T P^T (mma.sync m16n8k16, N = 8 query rows of one KV
@@ -565,24 +565,24 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && NG < 4 ? 3 : 2) kv4_
         const uint4 w = r < rows ? *reinterpret_cast<const uint4 *>(q + b * 32) : make_uint4(0, 0, 0, 0);
         qb[t][b][0] = w.x, qb[t][b][1] = w.y, qb[t][b][2] = w.z, qb[t][b][3] = w.w;
       }
-      if (!F16) {
-        // bf16 to fp16: divided by the power of two of the row's largest value, whose 8 bits fp16's 11 hold; values 2^-14 of it
-        // and less keep 2^-25 of it.  A row of zeros, or with an infinity or a NaN, is converted as it is.
-        uint32_t top = 0;
+      // To fp16, divided by the power of two of the row's largest value: bf16's 8 bits fit fp16's 11, and fp16 keeps its own (small
+      // rows too, of which a sixteenth would be subnormal); values 2^-14 of the largest and less keep 2^-25 of it, a sixteenth of
+      // them 2^-21.  A row of zeros, or with an infinity or a NaN, is converted as it is.
+      uint32_t most = 0;
 #pragma unroll
-        for (int b = 0; b < kWordsK; ++b)
+      for (int b = 0; b < kWordsK; ++b)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) top = max(top, max((qb[t][b][i] >> 7) & 0xffu, (qb[t][b][i] >> 23) & 0xffu));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = top == 0 || top == 255 ? 0 : int(top) - 127;
-        const float down = __uint_as_float(uint32_t(127 - (e > 126 ? 126 : e)) << 23);
-        back = g.sl / down;
+        for (int i = 0; i < 4; ++i) most = __vmaxu2(most, qb[t][b][i] & 0x7fff7fffu);
+      most = max(most & 0xffffu, most >> 16);
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      const int top = int(__float_as_uint(to_f32<F16>(most)) >> 23), e = top == 0 || top == 255 ? 0 : min(top - 127, 126);
+      const float down = __uint_as_float(uint32_t(127 - e) << 23);
+      back = g.sl / down;
 #pragma unroll
-        for (int b = 0; b < kWordsK; ++b)
+      for (int b = 0; b < kWordsK; ++b)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) qb[t][b][i] = pack_16x2<true>(lo_bf16(qb[t][b][i]) * down, hi_bf16(qb[t][b][i]) * down);
-      }
+        for (int i = 0; i < 4; ++i) qb[t][b][i] = pack_16x2<true>(lo_f32<F16>(qb[t][b][i]) * down, hi_f32<F16>(qb[t][b][i]) * down);
       float odd[NG];
 #pragma unroll
       for (int i = 0; i < NG; ++i) odd[i] = 0.f;

@@ -563,6 +563,22 @@ def test_cache_attention_of_flat_and_peaked_rows(page, dtype):
         near(o, *cache_attention(q, k, v, lens, 64, scale), DT[dtype], f"scale {scale}")
 
 
+@pytest.mark.parametrize("dtype,power", [("float16", -14), ("float16", 8), ("bfloat16", -100), ("bfloat16", 100)])
+def test_cache_attention_of_queries_far_from_one(dtype, power):
+    """Queries at the ends of their type's range (fp16: 2^-14 times the usual, partly subnormal), the scale making up for it: the
+    products are exact in powers of two, so the bound is that of usual queries."""
+    lens = [700, 65]
+    c, table, pool = cache_case(lens, 128, 16, 64, 1, dtype, 32)
+    k, v = rows_of(sum(lens), c, 33)
+    q = (torch.randn(2, 8, 128, generator=gen(34)) * 2.0 ** power).to(DT[dtype]).cuda()
+    books = [ints(lens), ints(table), pool]
+    launch(B.kv4_store(c, sum(lens)), [k, v, ints(starts(lens))] + books)
+    o = torch.zeros_like(q)
+    scale = 2.0 ** -power / math.sqrt(128)
+    launch(B.attention_kv4(c, 8, scale=scale), [q] + books + [o])
+    near(o, *cache_attention(q, k, v, lens, 64, scale), DT[dtype])
+
+
 def test_cache_attention_of_wide_values_in_fp16():
     """V scales of thousands times weights: no operand leaves fp16."""
     lens = [90]
