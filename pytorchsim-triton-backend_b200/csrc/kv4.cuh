@@ -5,12 +5,12 @@
 // a (c - 8) + (b + 8 a) and the score z = sum_g a_g (q . (c - 8))_g + (b_g + 8 a_g) sum(q)_g: the tensor core multiplies q by
 // small integers, exact in 16 bits, and the parameters enter in fp32, once per (key, group).  Likewise
 // O = sum_k (p a_g) (c - 8) + p (b_g + 8 a_g), with p a_g rounded to fp16 as the product's operand (2^-12 of what multiplies
-// |c - 8| <= 8) and the second sum kept per row in fp32.  Both products run in fp16 whatever the cache's type: a byte of two
+// |c - 8| <= 8; small ones: kKvTop) and the second sum kept per row in fp32.  Both products run in fp16 whatever the cache's type: a byte of two
 // codes becomes two fp16 operands by half a byte permute (0x64 above the byte: 1024 + lo + 16 hi), one mask-and-or
 // (1032 + 16 hi), one subtraction (lo - 8) and one fused multiply-add (hi - 8), two of them on the FMA pipe; bf16, with 7 bits
 // of mantissa, takes a shift more per pair, all on the half-rate ALU pipe, which bounded that form (63 % busy, 467 warp
 // instructions per 16 keys, 166 us of kernel at 4 slots of up to 131072 keys; this one 312 and 111 us).  Queries fit fp16 after division
-// by their row's power of two; the weights' V scales, of bf16 caches, by a power of two that follows the largest scale seen.  The operands are centred because a
+// by their row's power of two; the weights' V scales by a power of two that follows the largest scale seen.  The operands are centred because a
 // constant offset costs the sums their low bits: with 128 + c for V, 10^5 keys ended 2.4e-2 off (the tensor core truncates).
 //
 // The products have K and V as the 16-row operand: S^T = K q^T, O^T = V^T P^T (mma.sync m16n8k16, N = 8 query rows of one KV
@@ -362,12 +362,12 @@ __device__ __forceinline__ void split_offset(uint32_t x, uint32_t &lo, uint32_t 
   asm("sub.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(x), "r"(hi));
 }
 
-// How far (log2) a score may pass its row's reference before the reference moves.  The weight times the V scale is an fp16
-// operand: fp16 caches have scales up to 2 * 65504 / 15, and fp16 holds 2^2 times that, no 2^3; bf16 caches' scales are divided
-// by a power of two that keeps them to 2^6 (kKvScaleRoom), so that 2^14 bounds the product.
-template <bool F16>
-constexpr float kKvGrow = F16 ? 2.0f : 8.0f;
-constexpr int kKvScaleRoom = 6;
+// How far (log2) a score may pass its row's reference before the reference moves, and where (log2) the largest V scale seen is
+// brought by a power of two.  A weight times a scale is an fp16 operand, at most 2^(4 + 11); with the largest scale it is rounded by
+// 2^-12 of itself down to weights of 2^-24 (16 below the row's top score) and by 2^-35 of that scale behind.  A reference that moves
+// at 2^8 leaves a range of 2^-20 for the same times (64 slots of up to 8191 keys 65.2 us, 65.3 with 2^4), one at 2^2 costs the
+// rows that share a warp more moves (33 slots of up to 5000 keys, 16 rows a KV head of 64: 20.0 us, 18.6 with 2^4).
+constexpr int kKvGrow = 4, kKvTop = 15 - kKvGrow;
 
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t r;
@@ -614,8 +614,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && NG < 4 ? 3 : 2) kv4_
     }
     // nm: the rows' references (log2), negated, 0 before the first score; room: the unscaled score that moves it, -inf before the first.
     float nm[NT][2], room[NT][2], l[NT][2], corr[NT][2][NG], o[NT][D / 16][4];
-    float vdown = 1.f;                                      // power of two on the V scales (bf16 caches)
-    uint32_t vroom = 0;                                     // largest V scale (bits) it allows
+    float vdown = 1.f;                                      // power of two on the V scales
+    uint32_t vroom = 0;                                     // largest V scale (bits) it allows, 0 before the first
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -710,35 +710,29 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && NG < 4 ? 3 : 2) kv4_
 #pragma unroll
         for (int i = 0; i < 2; ++i)
           grow |= fmaxf(fmaxf(z[0][t][i], z[0][t][i + 2]), fmaxf(z[1][t][i], z[1][t][i + 2])) > room[t][i];
-      uint32_t vtop = 0;
-      if (!F16) {
-        vtop = vp[0][0][0];
+      uint32_t vtop = vp[0][0][0];
+#pragma unroll
+      for (int i = 0; i < NG; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) vtop = __vmaxu2(vtop, vp[k >> 1][k & 1][i]);
+      grow |= (vtop & 0xffffu) > vroom;
+      if (__any_sync(0xffffffffu, grow)) {
+        float f = 1.f;                                      // the V scales' power of two moves down
+        uint32_t top = 0;                                   // the largest finite scale
 #pragma unroll
         for (int i = 0; i < NG; ++i)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) vtop = __vmaxu2(vtop, vp[k >> 1][k & 1][i]);
-        vtop &= 0xffffu;
-        grow |= vtop > vroom;
-      }
-      if (__any_sync(0xffffffffu, grow)) {
-        float f = 1.f;                                      // the V scales' power of two moves down
-        if (!F16) {
-          uint32_t top = 0;                                 // the largest finite scale
-#pragma unroll
-          for (int i = 0; i < NG; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const uint32_t a = vp[k >> 1][k & 1][i] & 0xffffu;
-              if (a < 0x7f80u) top = max(top, a);
-            }
-          top = __reduce_max_sync(0xffffffffu, top);
-          if (top > vroom) {
-            const int e = min(max(int(top >> 7) - 126, -125), 126);            // 2^e > the scale
-            const float now = __uint_as_float(uint32_t(127 - e) << 23);
-            f = vroom == 0 ? 1.f : now / vdown;
-            vdown = now;
-            vroom = uint32_t(min(e + kKvScaleRoom + 127, 254)) << 7;
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t a = vp[k >> 1][k & 1][i] & 0xffffu;
+            if (a < (F16 ? 0x7c00u : 0x7f80u)) top = max(top, a);
           }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (top > vroom) {
+          const int e = max(int(__float_as_uint(to_f32<F16>(top)) >> 23) - 126, kKvTop - 126);   // 2^e > the scale, at most 2^128
+          const float now = __uint_as_float(uint32_t(127 + kKvTop - e) << 23);
+          f = vroom == 0 ? 1.f : now / vdown;
+          vdown = now;
+          vroom = !F16 ? uint32_t(e + 127) << 7 : e < -14 ? 1u << (e + 24) : uint32_t(e + 15) << 10;   // 2^e in the cache's type
         }
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -752,7 +746,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && NG < 4 ? 3 : 2) kv4_
             if (top > room[t][i] || (room[t][i] != -INFINITY && to > -nm[t][i])) {
               if (room[t][i] != -INFINITY) alpha = ex2_fast(-nm[t][i] - to);    // the first score: nothing to rescale
               nm[t][i] = -to;
-              room[t][i] = top + kKvGrow<F16> / sl[t][i];
+              room[t][i] = top + float(kKvGrow) / sl[t][i];
             }
             l[t][i] *= alpha;
 #pragma unroll
@@ -772,7 +766,7 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && NG < 4 ? 3 : 2) kv4_
 #pragma unroll
           for (int i = 0; i < NG; ++i) {
             a[i] = lo_f32<F16>(vp[h][k][i]), mid[i] = fmaf(8.f, a[i], hi_f32<F16>(vp[h][k][i]));
-            if (!F16) a[i] *= vdown;
+            a[i] *= vdown;
           }
 #pragma unroll
           for (int t = 0; t < NT; ++t) {

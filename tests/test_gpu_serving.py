@@ -579,6 +579,35 @@ def test_cache_attention_of_queries_far_from_one(dtype, power):
     near(o, *cache_attention(q, k, v, lens, 64, scale), DT[dtype])
 
 
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("size", [1.0, 0.02, 1e-3, 1e-4])
+@pytest.mark.parametrize("above,top", [(9, 0), (14, 0), (14, 1), (20, 0), (-20, 500)])
+def test_cache_attention_of_small_values_behind_one_key(dtype, size, above, top):
+    """One key's score `above` the others', its values `top` times theirs (-20, 500: far larger values with next to no weight); the
+    slots are as many as the launch has warps, so that each is one part.  A weight times a scale keeps fp16's digits down to 2^-24 of
+    the largest scale and is rounded by 2^-35 of it behind, which meets |code - 8| <= 8; the weights add up to 1 and more."""
+    n, slots, hkv, dim, some = 1100, 222, 8, 128, [0, 100, 221]
+    lens = [n] * slots
+    c, table, pool = cache_case(lens, dim, 64, 64, hkv, dtype, 30)
+    g = torch.Generator("cuda").manual_seed(31)
+    k = torch.randn(slots * n, hkv, dim, generator=g, device="cuda") * 0.5
+    v = (torch.rand(slots * n, hkv, dim, generator=g, device="cuda") + 1) * size
+    v *= torch.where(torch.arange(dim, device="cuda") % 2 == 0, 1.0, -1.0)
+    q = torch.randn(slots, hkv, dim, generator=g, device="cuda")
+    at = torch.arange(slots, device="cuda") * n + 3
+    k[at] = q * (above * math.sqrt(dim) / (q * q).sum(-1, keepdim=True))
+    v[at] *= top
+    k, v, q = (x.to(DT[dtype]) for x in (k, v, q))
+    books = [ints(lens), ints(table), pool]
+    launch(B.kv4_store(c, slots * n), [k, v, ints(starts(lens))] + books)
+    o = torch.zeros_like(q)
+    launch(B.attention_kv4(c, hkv), [q] + books + [o])
+    rows = [r for s in some for r in range(s * n, s * n + n)]
+    want, mag = cache_attention(q[some], k[rows], v[rows], [n] * 3, 64, 1 / math.sqrt(dim))
+    largest = float(S.quantise(v[rows], 64)[1].double().max())
+    near(o[some], want, mag + 8 * n * 2.0 ** -35 * largest / (torch.finfo(DT[dtype]).eps / 2), DT[dtype])
+
+
 def test_cache_attention_of_wide_values_in_fp16():
     """V scales of thousands times weights: no operand leaves fp16."""
     lens = [90]
