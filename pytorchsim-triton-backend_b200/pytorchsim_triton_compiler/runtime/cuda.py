@@ -10,6 +10,7 @@ GPUs, one host thread per GPU, and merges the written bytes exactly as merge_wor
 cannot give the answer, and the grid reruns on one GPU.  An argument read as well as written keeps the
 launch on one GPU (kernel_object.splittable)."""
 import concurrent.futures as cf
+import contextlib
 import os
 
 import numpy as np
@@ -68,20 +69,23 @@ _workspaces = {}
 
 def workspace_for(blob, device, stream=None):
     """Scratch a launch of `blob` wants on `device` (split-K partials, reduction partials), as a device tensor (or None).
-    It is kept per device and stream and grown on demand, so launches on two streams never share one; a launch that is
-    being captured gets one of its own from the capture's memory, which lives as long as the graph."""
+    It comes from the memory of the stream that the launch runs on (torch's current one by default), so what held it before
+    is ordered ahead of the launch.  It is kept per device and stream and grown on demand; launches on two streams never
+    share one.  A launch that is being captured gets one from the capture's memory, which lives as long as the graph:
+    later launches of its stream in that capture may be given the same, those of other branches never."""
     n = native.workspace_size(blob, device.index if device.index is not None else 0)
     if n <= 0:
         return None
     torch = _torch()
-    s = stream if stream is not None else torch.cuda.current_stream(device)
-    if torch.cuda.is_current_stream_capturing():
-        return torch.empty(int(n), dtype=torch.uint8, device=device)
-    key = (device, s.cuda_stream)
-    ws = _workspaces.get(key)
-    if ws is None or ws.numel() < n:
-        ws = _workspaces[key] = torch.empty(int(n), dtype=torch.uint8, device=device)
-        ws.record_stream(s)
+    current = torch.cuda.current_stream(device)
+    s = stream if stream is not None else current
+    with contextlib.nullcontext() if s.cuda_stream == current.cuda_stream else torch.cuda.stream(s):
+        if torch.cuda.is_current_stream_capturing():
+            return torch.empty(int(n), dtype=torch.uint8, device=device)
+        key = (device, s.cuda_stream)
+        ws = _workspaces.get(key)
+        if ws is None or ws.numel() < n:
+            ws = _workspaces[key] = torch.empty(int(n), dtype=torch.uint8, device=device)
     return ws
 
 

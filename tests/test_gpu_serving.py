@@ -916,6 +916,45 @@ def test_launches_on_two_streams_do_not_share_a_workspace():
         near(ts[-1], *want, torch.bfloat16)
 
 
+def test_launches_on_given_streams_have_workspaces_of_their_own():
+    """`stream=` with another stream current: eager, and as two branches of one capture that run at the same time."""
+    def case(seed, n):
+        c, table, pool = cache_case([n], 128, 16, 64, 1, "bfloat16", seed)
+        k, v = rows_of(n, c, seed)
+        q = torch.randn(1, 4, 128, generator=gen(seed)).to(torch.bfloat16).cuda()
+        books = [ints([n]), ints(table), pool]
+        launch(B.kv4_store(c, n), [k, v, ints([0, n])] + books)
+        return D.to_bytes(B.attention_kv4(c, 4)), [q] + books + [torch.zeros_like(q)], cache_attention(q, k, v, [n], 64, 1 / math.sqrt(128))
+    cases = [case(62, 20000), case(63, 17000)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+
+    def both():
+        for (blob, ts, _), s in zip(cases, streams):
+            for _ in range(4):
+                RC.launch_tensors(blob, ts, stream=s, sync=False)
+
+    def right():
+        torch.cuda.synchronize()
+        for _, ts, want in cases:
+            near(ts[-1], *want, torch.bfloat16)
+            ts[-1].zero_()
+        torch.cuda.synchronize()
+
+    torch.cuda.synchronize()
+    both()
+    right()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        both()
+        for s in streams:
+            torch.cuda.current_stream().wait_stream(s)
+    for _ in range(3):
+        g.replay()
+        right()
+
+
 def test_launch_tensors_can_be_captured():
     lens = [30, 200]
     q, k, v, q0, k0 = packed_case(lens, lens, 4, 2, 128, "bfloat16", 70)

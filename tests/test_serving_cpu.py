@@ -1,6 +1,8 @@
 """The serving operators without a GPU: their descriptors and refusals (ptsim_check), their access streams, and the
 64-bit oracle's own consistency (a token written into a record reads back as the values its codes stand for)."""
+import contextlib
 import json
+import types
 
 import pytest
 import torch
@@ -143,6 +145,49 @@ def test_builders_refuse_a_fused_projection_with_another_layout():
                  lambda: B.kv4_store(shape(), 7, fused_hq=4, head_major=True)):
         with pytest.raises(ValueError):
             make()
+
+
+class FakeCuda:
+    """What workspace_for asks of torch: the current stream, which streams are being captured, and memory by stream."""
+
+    def __init__(self):
+        self.cuda, self.uint8, self.now, self.captured, self.taken = self, torch.uint8, self.stream_of(1), set(), []
+
+    @staticmethod
+    def stream_of(n):
+        return types.SimpleNamespace(cuda_stream=n)
+
+    def current_stream(self, device=None):
+        return self.now
+
+    @contextlib.contextmanager
+    def stream(self, s):
+        held, self.now = self.now, s
+        yield
+        self.now = held
+
+    def is_current_stream_capturing(self):
+        return self.now.cuda_stream in self.captured
+
+    def empty(self, n, dtype, device):
+        self.taken.append(self.now.cuda_stream)
+        return torch.empty(n, dtype=dtype)
+
+
+def test_a_workspace_comes_from_the_stream_its_launch_runs_on(monkeypatch):
+    fake, device = FakeCuda(), torch.device("cuda", 0)
+    monkeypatch.setattr(RC, "_torch", lambda: fake)
+    monkeypatch.setattr(RC, "_workspaces", {})
+    blob = D.to_bytes(B.attention_kv4(shape(), 6))
+    own, side, third = RC.workspace_for(blob, device), fake.stream_of(2), fake.stream_of(3)
+    assert fake.taken == [1] and RC.workspace_for(blob, device) is own
+    other = RC.workspace_for(blob, device, side)
+    assert fake.taken == [1, 2] and other is not own and RC.workspace_for(blob, device, side) is other
+    fake.captured = {2, 3}                       # two branches of a capture, neither of them current
+    for branch in (side, third):
+        got = RC.workspace_for(blob, device, branch)
+        assert got is not own and got is not other and fake.taken[-1] == branch.cuda_stream
+    assert fake.now.cuda_stream == 1 and RC.workspace_for(blob, device) is own
 
 
 def test_graph_binds_device_tensors_only():
