@@ -336,7 +336,9 @@ typedef struct ptsim_pattn_params {
  *   c = d % 32 / 4, c ^ 4 for dim 128 where r & 2, nibble d % 4 + 4 (d % 64 / 32).
  *
  * KV4_STORE: token rows cu[s] .. cu[s + 1] of a (keys) and b (values) become the last tokens of slot s, which holds
- * lens[s] tokens with them (its pages are in the table already; a page that is written is held by that slot alone).  KV4_LOAD: the reverse, the last cu[s + 1] - cu[s]
+ * lens[s] tokens with them (its pages are in the table already; a page that is written is held by that slot alone).  After a
+ * GROW that was refused lens is what it was, and a store would write over the last tokens: a store that follows a GROW
+ * without a ptsim_sync between them takes its halt word.  KV4_LOAD: the reverse, the last cu[s + 1] - cu[s]
  * tokens of slot s into rows of a and b, scale * code + minimum in fp32 rounded to their type; rows of no slot are
  * left alone.  ATTN_KV4: a = q, b = o,
  * rows of one token per slot: query head h of slot s attends over the lens[s] cached tokens of KV head h / (hq / hkv); a
@@ -350,7 +352,8 @@ typedef struct ptsim_kv4_params {
   int64_t pages, page_size, max_pages, layers, layer;   /* page_size 16, 32, 64 or 128; dim 64 or 128; group 32, 64, 128 */
   int64_t a_off, a_row, a_head, b_off, b_row, b_head;
   int32_t a_arg, b_arg, cu_arg, lens_arg, table_arg, pool_arg;   /* cu_arg -1: ATTN_KV4 */
-  float scale, pad0;
+  float scale;
+  int32_t halt_arg_p1;    /* KV4_STORE: 1 + the argument of the halt word (PAGES); 0 when absent */
 } ptsim_kv4_params;
 
 /* PAGES: the bookkeeping of such a cache (any pool of layers x pages x page_bytes, page_bytes a multiple of 16).  refs
@@ -366,7 +369,10 @@ typedef struct ptsim_kv4_params {
  * (PTSIM_E_OOB); a negative aux of GROW, a slot listed twice in GROW, a target listed twice, not empty or also a source
  * (PTSIM_E_ARGS); a slot whose row cannot hold its pages or too few free pages (PTSIM_E_RESOURCE).  FREE and COMPACT record
  * such a slot (PTSIM_E_OOB) and pass over it.  A held table entry outside the pool is recorded (PTSIM_E_OOB) and not
- * counted, copied or moved.  One partition unit. */
+ * counted, copied or moved.
+ * The halt word (int32 [1]; halt_arg_p1: 1 + its argument, 0 when absent) ties launches that follow one another without a ptsim_sync: a GROW,
+ * FORK or COPY that is refused sets it to its code, and every PAGES and KV4_STORE launch that has it and finds it nonzero
+ * changes nothing.  The cache stays as it was before the refused launch until the caller clears the word.  One partition unit. */
 #define PTSIM_PAGES_GROW 1
 #define PTSIM_PAGES_FORK 2
 #define PTSIM_PAGES_COPY 3
@@ -375,7 +381,7 @@ typedef struct ptsim_kv4_params {
 #define PTSIM_PAGES_IDS 1024
 typedef struct ptsim_pages_params {
   int64_t n, slots, pages, page_size, max_pages, layers, page_bytes;
-  int32_t op, ids_arg, aux_arg, table_arg, lens_arg, refs_arg, pool_arg, pad0;
+  int32_t op, ids_arg, aux_arg, table_arg, lens_arg, refs_arg, pool_arg, halt_arg_p1;
 } ptsim_pages_params;
 
 typedef struct ptsim_reduce_params {

@@ -42,6 +42,7 @@ constexpr int kKvWarps = 4;
 struct Kv4Args {
   const uint8_t *pool;               // of the launch's layer
   const int32_t *lens, *table, *cu;
+  const int32_t *halt;               // (store) nonzero: write nothing; or null
   uint16_t *a, *b;                   // K and V, or q and o
   int64_t a_row, a_head, b_row, b_head;
   int64_t record;                    // bytes of one (page, KV head)
@@ -207,7 +208,7 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ 
   const uint32_t t = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int h0 = int(blockIdx.y) * (kHeads * HS) + lane / kLanes;
   pdl_enter();
-  if (t >= uint32_t(g.tokens)) return;
+  if (t >= uint32_t(g.tokens) || (g.halt != nullptr && *g.halt != 0)) return;
   const Kv4Lane<D, NG> me(lane);
   const uint16_t *src = me.is_v ? g.b + t * g.b_row : g.a + t * g.a_row;
   const int64_t step_h = me.is_v ? g.b_head : g.a_head;
@@ -992,6 +993,7 @@ int launch_kv4(const ptsim_desc &d, void *const *ptrs, void *ws, size_t ws_bytes
   g.lens = static_cast<const int32_t *>(ptrs[p.lens_arg]);
   g.table = static_cast<const int32_t *>(ptrs[p.table_arg]);
   g.cu = attn ? nullptr : static_cast<const int32_t *>(ptrs[p.cu_arg]);
+  g.halt = p.halt_arg_p1 == 0 ? nullptr : static_cast<const int32_t *>(ptrs[p.halt_arg_p1 - 1]);
   g.a = static_cast<uint16_t *>(ptrs[p.a_arg]) + p.a_off;
   g.b = static_cast<uint16_t *>(ptrs[p.b_arg]) + p.b_off;
   for (const void *q : {static_cast<const void *>(pool), static_cast<const void *>(g.a), static_cast<const void *>(g.b)})

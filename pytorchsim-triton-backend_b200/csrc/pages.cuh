@@ -22,11 +22,13 @@ struct PagesArgs {
   const int32_t *ids, *aux;
   int32_t *table, *lens, *refs;
   uint8_t *pool;
-  int32_t *head, *from, *to, *remap;  // workspace: [0] pages to copy (-1: refused), [1] used pages; [pages] each
+  int32_t *halt;                      // nonzero: change nothing; or null
+  int32_t *head, *from, *to, *remap;  // workspace: [0] pages to copy (-1: refused or halted), [1] used pages; [pages] each
   int64_t page_bytes;
   int32_t op, n, slots, pages, page_size, max_pages, layers;
 };
 
+__device__ __forceinline__ bool pages_halted(const PagesArgs &g) { return g.halt != nullptr && *g.halt != 0; }
 __device__ __forceinline__ int pages_held(const PagesArgs &g, int len) { return (len + g.page_size - 1) / g.page_size; }
 __device__ __forceinline__ bool pages_len_ok(const PagesArgs &g, int len) {
   return len >= 0 && len <= int64_t(g.max_pages) * g.page_size;
@@ -72,6 +74,10 @@ __global__ void __launch_bounds__(kPagesThreads) pages_plan_kernel(const __grid_
   const int i = threadIdx.x;
   if (i == 0) refused = 0, asked = 0;
   pdl_enter();
+  if (pages_halted(g)) {
+    if (i == 0) g.head[0] = -1;
+    return;
+  }
   if (g.op == PTSIM_PAGES_COMPACT) {
     // Used pages, then the k-th hole below their number and the k-th used page from it on.
     int used = 0, total;
@@ -173,7 +179,9 @@ __global__ void __launch_bounds__(kPagesThreads) pages_plan_kernel(const __grid_
   }
   if (args || oob || short_) {
     if (i == 0) {
-      record_status(oob ? PTSIM_E_OOB : args ? PTSIM_E_ARGS : PTSIM_E_RESOURCE);
+      const int why = oob ? PTSIM_E_OOB : args ? PTSIM_E_ARGS : PTSIM_E_RESOURCE;
+      record_status(why);
+      if (g.halt != nullptr) *g.halt = why;
       g.head[0] = -1;
     }
     return;
@@ -260,6 +268,7 @@ __global__ void __launch_bounds__(256) pages_apply_kernel(const __grid_constant_
 // One CTA per listed slot.
 __global__ void __launch_bounds__(256) pages_free_kernel(const __grid_constant__ PagesArgs g) {
   pdl_enter();
+  if (pages_halted(g)) return;
   const int id = g.ids[blockIdx.x];
   bool again = false;
   for (int j = threadIdx.x; j < int(blockIdx.x); j += 256) again |= g.ids[j] == id;
@@ -300,6 +309,7 @@ int launch_pages(const ptsim_desc &d, void *const *ptrs, void *ws, size_t ws_byt
   g.lens = ints(p.lens_arg);
   g.refs = ints(p.refs_arg);
   g.pool = p.pool_arg < 0 ? nullptr : static_cast<uint8_t *>(ptrs[p.pool_arg]);
+  g.halt = ints(p.halt_arg_p1 - 1);
   if (reinterpret_cast<uintptr_t>(g.pool) % 16 != 0) return fail(PTSIM_E_ARGS, "the pool is not 16-byte aligned");
   g.page_bytes = p.page_bytes;
   g.op = p.op;

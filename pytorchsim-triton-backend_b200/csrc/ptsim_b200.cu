@@ -195,6 +195,10 @@ static int check_kv4(const ptsim_desc &d) {
   const int dt = d.arg_dtype[q.a_arg];
   if ((dt != PTSIM_DT_BF16 && dt != PTSIM_DT_F16) || d.arg_dtype[q.b_arg] != dt)
     return fail(PTSIM_E_UNSUPPORTED, "a 4-bit cache stands for bf16 or fp16 values, one type throughout");
+  if (q.halt_arg_p1 != 0) {
+    if (d.kind != PTSIM_KIND_KV4_STORE) return fail(PTSIM_E_DESC, "a halt word of a launch that leaves the cache as it is");
+    if ((rc = check_ints(d, q.halt_arg_p1 - 1, 1, "the halt word"))) return rc;
+  }
   if (d.kind != PTSIM_KIND_KV4_STORE && q.a_arg == q.b_arg) return fail(PTSIM_E_DESC, "the 4-bit cache's output is an argument of its own");
   return PTSIM_OK;
 }
@@ -210,6 +214,7 @@ static int check_pages(const ptsim_desc &d) {
   if (rc || (rc = check_ints(d, q.refs_arg, q.pages, "the page counts"))) return rc;
   if (q.op != PTSIM_PAGES_COMPACT && (rc = check_ints(d, q.ids_arg, q.n, "the listed slots"))) return rc;
   if (q.op < PTSIM_PAGES_FREE && (rc = check_ints(d, q.aux_arg, q.n, "the second list"))) return rc;
+  if (q.halt_arg_p1 != 0 && (rc = check_ints(d, q.halt_arg_p1 - 1, 1, "the halt word"))) return rc;
   if (q.slots < 1 || q.pages < 1 || q.max_pages < 1) return fail(PTSIM_E_DESC, "a page operation on a cache without slots or pages");
   return PTSIM_OK;
 }

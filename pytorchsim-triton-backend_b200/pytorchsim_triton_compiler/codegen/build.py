@@ -167,16 +167,18 @@ def _kv4(kind, cache, specs, layer, **fields):
     return d
 
 
-def kv4_store(cache, tokens, layer=0, fused_hq=None, head_major=False):
+def kv4_store(cache, tokens, layer=0, fused_hq=None, head_major=False, halt=False):
     """New keys and values into a 4-bit cache: rows cu[s] .. cu[s + 1] become the last tokens of slot s, which holds lens[s]
     tokens with them.  Arguments k, v [tokens, hkv, dim], cu (int32 [slots + 1]), lens, table, pool; `fused_hq`: one
-    projection qkv [tokens, fused_hq + 2 hkv, dim] in the place of k and v; `head_major`: k is [hkv, tokens, dim]."""
+    projection qkv [tokens, fused_hq + 2 hkv, dim] in the place of k and v; `head_major`: k is [hkv, tokens, dim]; `halt`: a
+    last argument, the halt word of the page operations before it (int32 [1]): nothing is written if one was refused."""
     n = cache.hkv * cache.dim
     if fused_hq is not None and head_major:
         raise ValueError("a fused projection holds one token's q, k and v together")
     kv = [("qkv_ptr", cache.dtype, tokens * (fused_hq * cache.dim + 2 * n))] if fused_hq is not None else \
         [("k_ptr", cache.dtype, tokens * n), ("v_ptr", cache.dtype, tokens * n)]
-    d = _kv4(D.KV4_STORE, cache, kv + [("cu_ptr", "int32", cache.slots + 1)] + cache.books(), layer, tokens=tokens)
+    specs = kv + [("cu_ptr", "int32", cache.slots + 1)] + cache.books() + ([("halt_ptr", "int32", 1)] if halt else [])
+    d = _kv4(D.KV4_STORE, cache, specs, layer, tokens=tokens, halt_arg_p1=len(specs) if halt else 0)
     if fused_hq is not None:
         row = fused_hq * cache.dim + 2 * n
         _place(d.p.kv4, "a", 0, fused_hq * cache.dim, row, cache.dim)
@@ -211,11 +213,13 @@ def attention_kv4(cache, hq, layer=0, scale=None, fused=False):
     return d
 
 
-def _pages(op, cache, lists, pool):
+def _pages(op, cache, lists, pool, halt):
     specs = [(n, "int32", k) for n, k in lists] + [("table_ptr", "int32", cache.slots * cache.max_pages),
                                                    ("lens_ptr", "int32", cache.slots), ("refs_ptr", "int32", cache.pages)]
     if pool:
         specs.append(("pool_ptr", "uint8", cache.pool_bytes))
+    if halt:
+        specs.append(("halt_ptr", "int32", 1))
     d = D.new(D.PAGES, _args(specs), (1, 1, 1), units=1, unit_size=1)
     q, m = d.p.pages, len(lists)
     q.n = lists[0][1] if lists else 0
@@ -223,28 +227,30 @@ def _pages(op, cache, lists, pool):
         setattr(q, n, getattr(cache, n))
     q.op, q.ids_arg, q.aux_arg = D.PAGES_OP[op], 0 if m > 0 else -1, 1 if m > 1 else -1
     q.table_arg, q.lens_arg, q.refs_arg, q.pool_arg = m, m + 1, m + 2, m + 3 if pool else -1
+    q.halt_arg_p1 = len(specs) if halt else 0
     return d
 
 
-def pages_grow(cache, n):
-    """Room for add[i] more tokens in slot ids[i]: arguments ids, add (int32 [n]), table, lens, refs."""
-    return _pages("grow", cache, [("ids_ptr", n), ("add_ptr", n)], False)
+def pages_grow(cache, n, halt=False):
+    """Room for add[i] more tokens in slot ids[i]: arguments ids, add (int32 [n]), table, lens, refs.  `halt` (here and
+    below): a last argument, an int32 [1] that a refused grow or fork sets and that stops the launches which are given it."""
+    return _pages("grow", cache, [("ids_ptr", n), ("add_ptr", n)], False, halt)
 
 
-def pages_fork(cache, n, deep=False):
+def pages_fork(cache, n, deep=False, halt=False):
     """Empty slot dst[i] as a copy of slot src[i], sharing its full pages (`deep`: none): arguments src, dst (int32
     [n]), table, lens, refs, pool."""
-    return _pages("copy" if deep else "fork", cache, [("src_ptr", n), ("dst_ptr", n)], True)
+    return _pages("copy" if deep else "fork", cache, [("src_ptr", n), ("dst_ptr", n)], True, halt)
 
 
-def pages_free(cache, n):
+def pages_free(cache, n, halt=False):
     """Slots ids[i] give their pages back: arguments ids (int32 [n]), table, lens, refs."""
-    return _pages("free", cache, [("ids_ptr", n)], False)
+    return _pages("free", cache, [("ids_ptr", n)], False, halt)
 
 
-def pages_compact(cache):
+def pages_compact(cache, halt=False):
     """Used pages moved to the front of the pool: arguments table, lens, refs, pool."""
-    return _pages("compact", cache, [], True)
+    return _pages("compact", cache, [], True, halt)
 
 
 def gemv(N, K, b_kmajor=False, residual=False, out_dtype="bfloat16"):

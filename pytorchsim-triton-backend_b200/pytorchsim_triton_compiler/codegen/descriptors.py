@@ -178,7 +178,7 @@ class Kv4Params(C.Structure):
                                          "max_pages", "layers", "layer")] + \
                [(f"{x}_{n}", C.c_int64) for x in "ab" for n in ("off", "row", "head")] + \
                [(n, C.c_int32) for n in ("a_arg", "b_arg", "cu_arg", "lens_arg", "table_arg", "pool_arg")] + \
-               [("scale", C.c_float), ("pad0", C.c_float)]
+               [("scale", C.c_float), ("halt_arg_p1", C.c_int32)]
 
 
 PAGES_OP = {"grow": 1, "fork": 2, "copy": 3, "free": 4, "compact": 5}
@@ -188,7 +188,7 @@ PAGES_OP_NAME = {v: k for k, v in PAGES_OP.items()}
 class PagesParams(C.Structure):
     _fields_ = [(n, C.c_int64) for n in ("n", "slots", "pages", "page_size", "max_pages", "layers", "page_bytes")] + \
                [(n, C.c_int32) for n in ("op", "ids_arg", "aux_arg", "table_arg", "lens_arg", "refs_arg", "pool_arg",
-                                         "pad0")]
+                                         "halt_arg_p1")]
 
 
 class Params(C.Union):

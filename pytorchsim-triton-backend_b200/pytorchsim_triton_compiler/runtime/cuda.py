@@ -156,7 +156,8 @@ def written_args(desc):
         books = [p.pages.table_arg, p.pages.lens_arg, p.pages.refs_arg]
         if p.pages.op == D.PAGES_OP["compact"]:
             return [p.pages.table_arg, p.pages.refs_arg, p.pages.pool_arg]
-        return books + ([p.pages.pool_arg] if p.pages.pool_arg >= 0 else [])
+        halt = [p.pages.halt_arg_p1 - 1] if p.pages.halt_arg_p1 and p.pages.op != D.PAGES_OP["free"] else []
+        return books + ([p.pages.pool_arg] if p.pages.pool_arg >= 0 else []) + halt
     if k == D.INT_TABLE:
         return sorted({o.arg for o in list(p.itab.out)[:p.itab.nout]})
     raise CudaError(f"descriptor kind {k} ({D.KIND_NAME.get(k, 'unknown')}) has no known outputs")

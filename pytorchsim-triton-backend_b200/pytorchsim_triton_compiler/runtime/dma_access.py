@@ -265,6 +265,8 @@ def _kv4(d, names):
     dense = _rows_through([q.cu_arg], q.tokens * q.hkv, q.dim, names)
     pool = _rows_through([q.cu_arg, q.lens_arg, q.table_arg], q.tokens, token, names)
     store = d.kind == D.KV4_STORE
+    if q.halt_arg_p1:
+        out.append(_ints(q.halt_arg_p1 - 1, 1))
     return out + [(q.pool_arg, "write" if store else "read", pool), (q.a_arg, "read" if store else "write", dense),
                   (q.b_arg, "read" if store else "write", dense)]
 
@@ -278,6 +280,10 @@ def _page_books(d, names):
         out.append(_ints(arg, n))
         if arg != q.lens_arg or q.op != D.PAGES_OP["compact"]:
             out.append((arg, "write", _box(0, [(n, 1)])))
+    if q.halt_arg_p1:
+        out.append(_ints(q.halt_arg_p1 - 1, 1))
+        if q.op not in (D.PAGES_OP["free"], D.PAGES_OP["compact"]):
+            out.append((q.halt_arg_p1 - 1, "write", _box(0, [(1, 1)])))
     if q.pool_arg >= 0:
         moved = _rows_through([a for a, _ in tables], q.pages * q.layers, q.page_bytes, names)
         out += [(q.pool_arg, "read", moved), (q.pool_arg, "write", moved)]

@@ -896,6 +896,76 @@ def test_a_captured_decode_step_grows_its_slots():
     assert state["lens"].tolist() == [40] * 4 and int((state["refs"] > 0).sum()) == 12
 
 
+def test_a_captured_decode_step_that_runs_out_of_pages_leaves_the_cache():
+    """Four slots of one page each and one page to spare: the step that needs four more is refused, and from there the replays change
+    nothing; with a slot freed and the halt word cleared they go on, and every token is where the dense history has it."""
+    slots, hq, hkv = 4, 8, 2
+    c = B.kv4_cache(slots=slots, max_pages=4, pages=5, hkv=hkv, dim=128, page_size=16, group=64)
+    state = {"ids": ints([0, 1, 2, 3]), "one": ints([1] * 4), "table": ints([[-1] * 4] * 4), "lens": ints([0] * 4), "refs": ints([0] * 5),
+             "halt": ints([0]), "pool": torch.zeros(c.pool_bytes, dtype=torch.uint8, device="cuda"), "cu": ints(range(5)),
+             "qkv": torch.zeros(slots, hq + 2 * hkv, 128, dtype=torch.bfloat16, device="cuda"),
+             "o": torch.zeros(slots, hq, 128, dtype=torch.bfloat16, device="cuda")}
+    g = Graph("cuda:0")
+    for name, t in state.items():
+        g.bind(name, t)
+    g.add("grow", D.to_bytes(B.pages_grow(c, slots, halt=True)), ["ids", "one", "table", "lens", "refs", "halt"])
+    g.add("store", D.to_bytes(B.kv4_store(c, slots, fused_hq=hq, halt=True)), ["qkv", "cu", "lens", "table", "pool", "halt"])
+    g.add("attend", D.to_bytes(B.attention_kv4(c, hq, fused=True)), ["qkv", "lens", "table", "pool", "o"])
+    past, r, stream = [], gen(91), torch.cuda.current_stream().cuda_stream
+
+    def step():
+        state["qkv"].copy_(torch.randn(slots, hq + 2 * hkv, 128, generator=r).to(torch.bfloat16))
+        past.append(state["qkv"].clone())
+        g.run() if g.cuda_graph else g.capture()
+
+    for _ in range(16):
+        step()
+    native.sync(stream)
+    books = [state[n].clone() for n in ("table", "lens", "refs", "pool")]
+    for _ in range(3):                                       # refused once, then halted
+        step()
+    with pytest.raises(native.ExecutorError) as e:
+        native.sync(stream)
+    assert e.value.code == D.E_RESOURCE and state["halt"].tolist() == [D.E_RESOURCE]
+    for t, n in zip(books, ("table", "lens", "refs", "pool")):
+        assert torch.equal(t, state[n]), n
+    native.sync(stream)                                      # the halted replays recorded nothing more
+    del past[16:]
+    launch(B.pages_free(c, 1, halt=True), [ints([3])] + [state[n] for n in ("table", "lens", "refs", "halt")])
+    assert state["lens"].tolist() == [16] * 4                # halted as well
+    launch(B.pages_free(c, 3), [ints([1, 2, 3])] + [state[n] for n in ("table", "lens", "refs")])
+    state["halt"].zero_()
+    step()
+    native.sync(stream)
+    assert state["lens"].tolist() == [17, 1, 1, 1]
+    rows = torch.cat([torch.stack(past)[:, 0], past[-1][1:]])
+    q, k, v = (x.contiguous() for x in rows.split([hq, hkv, hkv], 1))
+    near(state["o"], *cache_attention(past[-1][:, :hq], k, v, [17, 1, 1, 1], 64, 1 / math.sqrt(128)), torch.bfloat16)
+
+
+def test_a_refused_fork_halts_what_follows():
+    a = Live(slots=5, width=4, pages=7, page=16)
+    a.grow([0, 1], [40, 20])                                 # 3 + 2 pages of 7
+    halt = ints([0])
+    lists = lambda *x: [ints(i) for i in x] + a.books()
+    RC.launch_tensors(D.to_bytes(B.pages_fork(a.c, 1, deep=True, halt=True)), lists([0], [2]) + [a.pool, halt], sync=False)   # 3 pages of 2
+    k, v = rows_of(2, a.c, 3)
+    k, v = (x[:, :a.c.hkv].contiguous() for x in (k, v))
+    for desc, ts in ((B.pages_fork(a.c, 1, halt=True), lists([1], [3]) + [a.pool, halt]), (B.pages_grow(a.c, 1, halt=True), lists([1], [1]) + [halt]),
+                     (B.kv4_store(a.c, 2, halt=True), [k, v, ints([0, 1, 2, 2, 2, 2]), a.lens, a.table, a.pool.flatten(), halt]),
+                     (B.pages_free(a.c, 2, halt=True), lists([0, 1]) + [halt]), (B.pages_compact(a.c, halt=True), a.books() + [a.pool, halt])):
+        RC.launch_tensors(D.to_bytes(desc), ts, sync=False)
+    with pytest.raises(native.ExecutorError) as e:
+        native.sync(torch.cuda.current_stream().cuda_stream)
+    assert e.value.code == D.E_RESOURCE and halt.tolist() == [D.E_RESOURCE]
+    a.same()
+    halt.zero_()
+    launch(B.pages_fork(a.c, 1, halt=True), lists([1], [3]) + [a.pool, halt])
+    a.want.fork([1], [3])
+    a.same()
+    assert not halt.any()
+
+
 def test_launches_on_two_streams_do_not_share_a_workspace():
     def case(seed, n):
         c, table, pool = cache_case([n], 128, 16, 64, 1, "bfloat16", seed)

@@ -129,6 +129,39 @@ def test_page_refusals(make, fields, code):
     assert _code(_with(make(shape()), "pages", **fields)) == code
 
 
+def halted_builders():
+    c = shape()
+    return [B.kv4_store(c, 7, halt=True), B.kv4_store(c, 7, fused_hq=4, halt=True), B.pages_grow(c, 2, halt=True), B.pages_fork(c, 2, halt=True),
+            B.pages_fork(c, 2, deep=True, halt=True), B.pages_free(c, 2, halt=True), B.pages_compact(c, halt=True)]
+
+
+@pytest.mark.parametrize("i", range(7))
+def test_a_halt_word_is_the_last_argument(i):
+    desc, names = halted_builders()[i], [f"a{k}" for k in range(16)]
+    native.check(D.to_bytes(desc))
+    last = desc.nargs - 1
+    p, which = (desc.p.pages, "pages") if desc.kind == D.PAGES else (desc.p.kv4, "kv4")
+    assert p.halt_arg_p1 == desc.nargs and desc.arg_numel[last] == 1
+    sets = desc.kind == D.PAGES and p.op in (D.PAGES_OP["grow"], D.PAGES_OP["fork"], D.PAGES_OP["copy"])
+    assert (last in RC.written_args(desc)) == sets
+    streams = dma_access.streams(desc, 0, 1, names)
+    assert {s["arg"] for s in streams} == set(names[:desc.nargs])
+    assert {s["arg"] for s in streams if s["dir"] == "write"} == {names[k] for k in RC.written_args(desc)}
+    assert _code(_with(desc, which, halt_arg_p1=desc.nargs + 1)) == D.E_DESC
+    assert _code(_with(desc, which, halt_arg_p1=-1)) == D.E_DESC
+    desc = halted_builders()[i]
+    desc.arg_dtype[last] = D.DTYPE_CODE["int64"]
+    assert _code(desc) == D.E_UNSUPPORTED
+    desc = halted_builders()[i]
+    desc.arg_numel[last] = 0
+    assert _code(desc) == D.E_OOB
+
+
+def test_reading_launches_take_no_halt_word():
+    for desc in (B.kv4_load(shape(), 7), B.attention_kv4(shape(), 6)):
+        assert _code(_with(desc, "kv4", halt_arg_p1=2)) == D.E_DESC
+
+
 def test_launches_refuse_a_small_workspace_and_null_pointers_before_any_gpu():
     assert native.workspace_size(D.to_bytes(B.attention_kv4(shape(), 6))) > 0
     assert native.workspace_size(D.to_bytes(B.pages_fork(shape(), 2))) == 4 * (4 + 3 * 9)
