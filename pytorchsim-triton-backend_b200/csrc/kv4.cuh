@@ -404,8 +404,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && NG < 4 ? 3 : 2) kv4_
   uint8_t *ring = smem + (threadIdx.x >> 5) * kKvStages * kStage;
   uint64_t *full = reinterpret_cast<uint64_t *>(smem + kKvWarps * kKvStages * kStage) + (threadIdx.x >> 5) * kKvStages;
   int32_t *good = reinterpret_cast<int32_t *>(smem + kKvWarps * kKvStages * (kStage + 8)) + (threadIdx.x >> 5) * kKvStages;
-  int32_t *before = reinterpret_cast<int32_t *>(smem + kKvWarps * kKvStages * (kStage + 12));   // [slots + 1] units of an item before a slot
-  __shared__ int32_t sums[2 * kKvWarps];
+  int32_t *sums = reinterpret_cast<int32_t *>(smem + kKvWarps * kKvStages * (kStage + 12));   // [2 * kKvWarps]
+  int32_t *before = sums + 2 * kKvWarps;                    // [slots + 1] units of an item before a slot
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gq = lane >> 2, qd = lane & 3;
   const uint32_t wl = g.stall ? kTestWaitUs : kWaitUs;
   if (lane == 0) {
@@ -940,11 +940,19 @@ __global__ void __launch_bounds__(128) kv4_merge_kernel(const __grid_constant__ 
       make_uint2(pack_16x2<F16>(O.x * inv, O.y * inv), pack_16x2<F16>(O.z * inv, O.w * inv));
 }
 
-// Workers of a launch: one warp each, as many as are resident at once.
-// Warps of the attention: three CTAs an SM (168 registers a thread), two where 16 query heads or four groups of a head dimension take
-// more (64 slots of up to 8191 keys, groups of 32 at D 128: 83 us with two CTAs and 213 registers, 116 with three and spills).
+// Shared memory of a CTA of the attention: the warps' rings with their barriers and flags, the scan's sums, 6 bytes a slot.
+constexpr int kv4_smem(int dim, int group, int slots) {
+  return kKvWarps * kKvStages * (kKvTile * (dim + 8 * (dim / group)) + 12) + 8 * kKvWarps + 16 + 6 * (slots + 1);
+}
+
+// Workers of the attention: one warp each, as many as are resident at once.  By registers three CTAs an SM (168 a thread), two where
+// 16 query heads or four groups of a head dimension take more (64 slots of up to 8191 keys, groups of 32 at D 128: 83 us with two CTAs
+// and 213 registers, 116 with three and spills); by the SM's 228 KB, of which a CTA takes 1 KB and up to 128 bytes beside its own, two
+// from 466 slots on at D 128 in groups of 64 (1024 slots of up to 1000 keys: 184 us, 235 when cut for three).
 static int kv4_workers(const ptsim_kv4_params &p, int sm_count) {
-  return sm_count * (p.hq / p.hkv <= 8 && p.dim / p.group < 4 ? 3 : 2) * kKvWarps;
+  const int by_registers = p.hq / p.hkv <= 8 && p.dim / p.group < 4 ? 3 : 2;
+  const int by_memory = (228 << 10) / (kv4_smem(int(p.dim), int(p.group), int(p.slots)) + 1152);
+  return sm_count * (by_memory < by_registers ? by_memory : by_registers) * kKvWarps;
 }
 
 int64_t kv4_workspace(const ptsim_desc &d, int sm_count) {
@@ -955,9 +963,8 @@ int64_t kv4_workspace(const ptsim_desc &d, int sm_count) {
 template <int D, int NG, int NT, bool F16>
 static int run_kv4_attn(const Kv4Args &g, const LaunchCtx &c) {
   constexpr auto kern = kv4_attn_kernel<D, NG, NT, F16>;
-  constexpr int fixed = kKvWarps * kKvStages * (kKvTile * (D + 8 * NG) + 12) + 16;   // 6 bytes a slot follow
-  PTSIM_CUDA((smem_limit_once<kern>(fixed + 6 * (PTSIM_KV4_SLOTS + 1), c.device)));
-  PTSIM_CUDA(launch_pdl(kern, dim3(unsigned(g.workers / kKvWarps)), dim3(kKvWarps * 32), fixed + 6 * (g.slots + 1), c.stream, g));
+  PTSIM_CUDA((smem_limit_once<kern>(kv4_smem(D, D / NG, PTSIM_KV4_SLOTS), c.device)));
+  PTSIM_CUDA(launch_pdl(kern, dim3(unsigned(g.workers / kKvWarps)), dim3(kKvWarps * 32), kv4_smem(D, D / NG, g.slots), c.stream, g));
   const int rows = g.per < 16 ? g.per : 16;
   PTSIM_CUDA(launch_pdl(kv4_merge_kernel<D, F16>, dim3(unsigned(g.slots * g.hkv * g.rb), unsigned(ceil_div(rows * D, 128))), dim3(128), 0,
                         c.stream, g));

@@ -497,6 +497,25 @@ def test_cache_attention(dim, page, group, hkv, per, dtype, lens):
         assert n or not o[s].any()
 
 
+@pytest.mark.parametrize("slots,dim,group,dtype", [(129, 128, 64, "bfloat16"), (464, 128, 64, "bfloat16"), (600, 128, 64, "bfloat16"),
+                                                   (600, 64, 32, "float16"), (4096, 128, 32, "bfloat16"), (4096, 64, 64, "float16")])
+def test_cache_attention_of_many_slots(slots, dim, group, dtype):
+    """More slots than a CTA has threads: each sums a run of them.  Some hold nothing, runs of empty ones among them."""
+    lens = [(37 * i * i + 11 * i) % 150 if i % 50 < 45 else 0 for i in range(slots)]
+    c, table, pool = cache_case(lens, dim, 16, group, 1, dtype, slots)
+    k, v = rows_of(sum(lens), c, 24)
+    q = torch.randn(slots, 3, dim, generator=gen(25)).to(DT[dtype]).cuda()
+    books = [ints(lens), ints(table), pool]
+    launch(B.kv4_store(c, sum(lens)), [k, v, ints(starts(lens))] + books)
+    o = torch.full_like(q, 7.0)
+    launch(B.attention_kv4(c, 3), [q] + books + [o])
+    some = [s for s in range(slots) if s % 41 == 0 or s > slots - 60]
+    at = starts(lens)
+    rows = [r for s in some for r in range(at[s], at[s + 1])]
+    near(o[some], *cache_attention(q[some], k[rows], v[rows], [lens[s] for s in some], group, 1 / math.sqrt(dim)), DT[dtype])
+    assert not o[[s for s in range(slots) if not lens[s]]].any() and bool((o != 7).all())
+
+
 @pytest.mark.parametrize("dtype,page", [("bfloat16", 16), ("float16", 64)])
 def test_cache_attention_of_a_long_context(dtype, page):
     """100000 keys, whose weights average out: the result is 2^-8 of the values, and its error has to follow."""

@@ -129,6 +129,18 @@ def test_page_refusals(make, fields, code):
     assert _code(_with(make(shape()), "pages", **fields)) == code
 
 
+@pytest.mark.parametrize("slots", [1, 64, 464, 465, 600, 1024, 4096])
+@pytest.mark.parametrize("dim,group,per", [(128, 64, 4), (128, 128, 8), (128, 32, 4), (64, 64, 3), (64, 32, 12)])
+def test_cache_attention_cuts_its_work_for_the_warps_an_sm_holds(slots, dim, group, per):
+    """The workspace has two parts a warp, for as many CTAs of four warps as fit the 228 KB of an SM's shared memory: a tile ring of two
+    stages a warp, 12 bytes a stage, 6 bytes a slot, 1 KB that the hardware keeps."""
+    c = shape(dim=dim, group=group, hkv=1, slots=slots)
+    floats = native.workspace_size(D.to_bytes(B.attention_kv4(c, per))) // 4 - slots - 1
+    ctas, rest = divmod(floats, 2 * 4 * 148 * 16 * (dim + 2))
+    smem = 8 * (64 * (dim + 8 * (dim // group)) + 12) + 32 + 6 * (slots + 1) + 1024
+    assert rest == 0 and 2 <= ctas <= 3 and ctas * smem <= 228 * 1024
+
+
 def halted_builders():
     c = shape()
     return [B.kv4_store(c, 7, halt=True), B.kv4_store(c, 7, fused_hq=4, halt=True), B.pages_grow(c, 2, halt=True), B.pages_fork(c, 2, halt=True),
