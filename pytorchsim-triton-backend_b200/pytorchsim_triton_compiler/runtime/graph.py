@@ -40,7 +40,7 @@ class Graph:
         if not tensor.is_cuda or not tensor.is_contiguous() or tensor.device.index != (self.device.index or 0):
             raise ValueError(f"buffer {name}: a contiguous tensor on {self.device} is required")
         held = self.buffers.get(name)
-        if held is not None and held.data_ptr() != tensor.data_ptr():
+        if held is not None and (held.data_ptr() != tensor.data_ptr() or held.numel() != tensor.numel() or held.dtype != tensor.dtype):
             raise ValueError(f"buffer {name} exists already")
         self.buffers[name] = tensor
         return name

@@ -241,6 +241,29 @@ def test_graph_binds_device_tensors_only():
         g.bind("x", torch.zeros(4))
 
 
+class OnDevice(torch.Tensor):
+    """A host tensor that says it lies on cuda:0 (what the launch boundary looks at; nothing is launched)."""
+    is_cuda = True
+
+    @property
+    def device(self):
+        return torch.device("cuda", 0)
+
+
+def on_device(*shape, dtype):
+    return torch.zeros(*shape, dtype=dtype).as_subclass(OnDevice)
+
+
+def test_a_bound_buffer_keeps_its_size_and_type():
+    g, t = Graph("cuda:0"), on_device(8, dtype=torch.int32)
+    g.bind("x", t)
+    g.bind("x", t)
+    for other in (t[:4], t.view(torch.float32), on_device(8, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            g.bind("x", other)
+    assert g.buffers["x"] is t
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_quantisation_is_within_its_step(dtype, group):
