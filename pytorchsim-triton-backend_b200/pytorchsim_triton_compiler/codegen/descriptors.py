@@ -31,6 +31,13 @@ def kind_name(kind):
 # Element types (PTSIM_DT_*), keyed by kernel.json dtype names (contract/kernel_object.py NP_DTYPE keys).
 DTYPE_CODE = {"float32": 0, "bfloat16": 1, "float16": 2, "int32": 3, "int64": 4, "int16": 5, "int8": 6,
               "uint8": 7, "float64": 8, "bool": 6}
+DTYPE_BYTES = (4, 2, 2, 4, 8, 2, 1, 1, 8)   # by code
+
+
+def element_size(d, i):
+    """Bytes of an element of argument `i` of descriptor `d`, 0 for a type that no launch takes."""
+    return DTYPE_BYTES[d.arg_dtype[i]] if 0 <= d.arg_dtype[i] < len(DTYPE_BYTES) else 0
+
 
 # Vector-unit opcodes (PTSIM_OP_*).
 OP = {"load": 1, "const": 2, "add": 3, "sub": 4, "mul": 5, "div": 6, "neg": 7, "exp": 8, "rsqrt": 9,

@@ -105,6 +105,8 @@ def launch_tensors(blob, tensors, lo=0, hi=None, stream=None, sync=True):
             raise CudaError(f"argument {i} is not contiguous; kernel.json tensors are flat")
         if t.numel() != desc.arg_numel[i]:
             raise CudaError(f"argument {i} holds {t.numel()} elements, the descriptor {desc.arg_numel[i]}")
+        if D.element_size(desc, i) not in (0, t.element_size()):
+            raise CudaError(f"argument {i} is {t.dtype}, the descriptor has elements of {D.element_size(desc, i)} bytes")
         dev = t.device if dev is None else dev
         if t.device != dev:
             raise CudaError("every argument of one launch is on one device")

@@ -47,7 +47,7 @@ class Graph:
 
     def add(self, name, blob, bufs, owners=None):
         """Append a launch of descriptor `blob` whose tensor arguments are the buffers `bufs`, in the
-        descriptor's argument order; every buffer must exist with the descriptor's element count.  `owners`
+        descriptor's argument order; every buffer must exist with the descriptor's element count and size.  `owners`
         = (device pointers, rows): a GEMM whose output rows go to their owner ranks in blocks of `rows`
         (native.launch_rows_to_owners) instead of into its output buffer."""
         d = D.from_bytes(blob)
@@ -57,6 +57,8 @@ class Graph:
             t = self.buffers[b]
             if t.numel() != d.arg_numel[i]:
                 raise ValueError(f"{name}: buffer {b} holds {t.numel()} elements, argument {i} wants {d.arg_numel[i]}")
+            if D.element_size(d, i) not in (0, t.element_size()):
+                raise ValueError(f"{name}: buffer {b} is {t.dtype}, argument {i} has elements of {D.element_size(d, i)} bytes")
         native.check(blob)
         ws = None
         n = native.workspace_size(blob, self.device.index or 0)

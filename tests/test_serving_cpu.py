@@ -264,6 +264,22 @@ def test_a_bound_buffer_keeps_its_size_and_type():
     assert g.buffers["x"] is t
 
 
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int16])
+def test_tensors_of_another_element_size_are_refused(dtype):
+    """int64 lengths, as torch makes them, are not the int32 ones a launch reads."""
+    c = shape()
+    desc = B.pages_free(c, 2)
+    ts = [on_device(n, dtype=torch.int32) for n in (2, c.slots * c.max_pages, c.slots, c.pages)]
+    ts[2] = on_device(c.slots, dtype=dtype)
+    with pytest.raises(RC.CudaError, match="argument 2"):
+        RC.launch_tensors(D.to_bytes(desc), ts)
+    g = Graph("cuda:0")
+    for n, t in zip(("ids", "table", "lens", "refs"), ts):
+        g.bind(n, t)
+    with pytest.raises(ValueError, match="lens"):
+        g.add("free", D.to_bytes(desc), ["ids", "table", "lens", "refs"])
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_quantisation_is_within_its_step(dtype, group):
