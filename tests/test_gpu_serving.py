@@ -671,6 +671,19 @@ def test_cache_attention_takes_a_fused_projection():
     assert torch.equal(a, b)
 
 
+def test_attention_without_any_key():
+    """No key row at all, and a cache without pages: every query gives zeros."""
+    q = torch.randn(200, 4, 64, generator=gen(93)).to(torch.bfloat16).cuda()
+    none = torch.empty(0, dtype=torch.bfloat16, device="cuda")
+    o = torch.full_like(q, 7.0)
+    launch(B.attention_packed(200, 2, 4, 2, 64, k_tokens=0), [q, none, none, ints([0, 150, 200]), ints([0, 0, 0]), o])
+    assert not o.any()
+    c = B.kv4_cache(slots=3, max_pages=0, pages=0, hkv=2, dim=64)
+    o = torch.full_like(q[:3], 7.0)
+    launch(B.attention_kv4(c, 4), [q[:3].contiguous(), ints([0, 0, 0]), ints([]), torch.empty(0, dtype=torch.uint8, device="cuda"), o])
+    assert not o.any()
+
+
 # --------------------------------------------------------------------------------------------------------------------
 # Page bookkeeping
 # --------------------------------------------------------------------------------------------------------------------
@@ -960,6 +973,22 @@ def test_a_captured_decode_step_that_runs_out_of_pages_leaves_the_cache():
     rows = torch.cat([torch.stack(past)[:, 0], past[-1][1:]])
     q, k, v = (x.contiguous() for x in rows.split([hq, hkv, hkv], 1))
     near(state["o"], *cache_attention(past[-1][:, :hq], k, v, [17, 1, 1, 1], 64, 1 / math.sqrt(128)), torch.bfloat16)
+
+
+def test_a_failure_is_raised_by_the_next_synchronisation_and_once():
+    """Of whichever operator: the launches after it run, and give what they always give."""
+    a = Live(slots=2, width=2, pages=1, page=16)
+    RC.launch_tensors(D.to_bytes(B.pages_grow(a.c, 1)), [ints([0]), ints([17])] + a.books(), sync=False)   # two pages of one
+    q, k, v, q0, k0 = packed_case([40], [40], 2, 1, 64, "bfloat16", 92)
+    o, again = torch.zeros_like(q), torch.zeros_like(q)
+    blob = D.to_bytes(B.attention_packed(40, 1, 2, 1, 64))
+    with pytest.raises(native.ExecutorError) as e:
+        RC.launch_tensors(blob, [q, k, v, ints(q0), o])
+    assert e.value.code == D.E_RESOURCE
+    RC.launch_tensors(blob, [q, k, v, ints(q0), again])
+    near(o, *dense(q, k, v, [40], [40], q0, k0, 1 / 8), torch.bfloat16)
+    assert torch.equal(o, again)
+    a.same()
 
 
 def test_a_refused_fork_halts_what_follows():
