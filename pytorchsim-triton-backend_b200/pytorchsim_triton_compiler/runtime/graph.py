@@ -72,18 +72,17 @@ class Graph:
     def run(self, stream=None, sync=False):
         """Enqueue every launch in order on `stream` (torch's current stream by default)."""
         torch = self.torch
+        at = self.device.index or 0
+        if torch.cuda.current_device() != at:    # launches and the status word are the current device's
+            with torch.cuda.device(at):
+                return self.run(stream, sync)
         s = stream or torch.cuda.current_stream(self.device)
         if self.cuda_graph is not None and stream is None:
             self.cuda_graph.replay()
         else:
             ptr = s.cuda_stream
-            if torch.cuda.current_device() == (self.device.index or 0):
-                for i in range(len(self.steps)):
-                    self._launch(i, ptr)
-            else:
-                with torch.cuda.device(self.device):
-                    for i in range(len(self.steps)):
-                        self._launch(i, ptr)
+            for i in range(len(self.steps)):
+                self._launch(i, ptr)
         if sync:
             native.sync(s.cuda_stream)
 
@@ -103,7 +102,7 @@ class Graph:
     def capture(self):
         """Capture the launch sequence into a CUDA graph (replayed by run())."""
         torch = self.torch
-        native.init(self.device.index or 0)
+        native.prepare(self.device.index or 0)
         self.run(sync=True)   # first use of every kernel outside the capture
         g = torch.cuda.CUDAGraph()
         s = torch.cuda.Stream(self.device)

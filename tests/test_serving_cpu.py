@@ -264,6 +264,32 @@ def test_a_bound_buffer_keeps_its_size_and_type():
     assert g.buffers["x"] is t
 
 
+@pytest.mark.parametrize("current", [0, 1])
+def test_a_graph_runs_and_synchronises_on_its_own_device(current, monkeypatch):
+    class Cuda:
+        now = current
+
+        def current_device(self):
+            return self.now
+
+        @contextlib.contextmanager
+        def device(self, d):
+            held, self.now = self.now, d
+            yield
+            self.now = held
+
+        def current_stream(self, device):
+            return types.SimpleNamespace(cuda_stream=7)
+
+    g, cuda, seen = Graph("cuda:0"), Cuda(), []
+    g.torch = types.SimpleNamespace(cuda=cuda)
+    g.steps = ["a step"]
+    monkeypatch.setattr(g, "_launch", lambda i, stream: seen.append(("launch", cuda.now, stream)))
+    monkeypatch.setattr(native, "sync", lambda stream: seen.append(("sync", cuda.now, stream)))
+    g.run(sync=True)
+    assert seen == [("launch", 0, 7), ("sync", 0, 7)] and cuda.now == current
+
+
 @pytest.mark.parametrize("dtype", [torch.int64, torch.int16])
 def test_tensors_of_another_element_size_are_refused(dtype):
     """int64 lengths, as torch makes them, are not the int32 ones a launch reads."""
