@@ -9,7 +9,7 @@
 // codes becomes two fp16 operands by half a byte permute (0x64 above the byte: 1024 + lo + 16 hi), one mask-and-or
 // (1032 + 16 hi), one subtraction (lo - 8) and one fused multiply-add (hi - 8), two of them on the FMA pipe; bf16, with 7 bits
 // of mantissa, takes a shift more per pair, all on the half-rate ALU pipe, which bounded that form (63 % busy, 467 warp
-// instructions per 16 keys, 166 us of kernel at 4 slots of up to 131072 keys; this one 312 and 111 us).  Queries fit fp16 after division
+// instructions per 16 keys, 166 us of kernel at 4 slots of up to 131072 keys; this one 310 and 111 us).  Queries fit fp16 after division
 // by their row's power of two; the weights' V scales by a power of two that follows the largest scale seen.  The operands are centred because a
 // constant offset costs the sums their low bits: with 128 + c for V, 10^5 keys ended 2.4e-2 off (the tensor core truncates).
 //
@@ -20,9 +20,10 @@
 // without bank conflicts give words whose nibbles are the fragments.
 //
 // Bound: HBM, (D + 8 D / group) bytes per key and KV head (144 at D 128, group 64: 3.5 times fewer than bf16), and before
-// it the issue slots of the unpacking (60 % busy with three warps per scheduler, ALU 47 %; a fourth warp, at 128 registers,
-// changed nothing).  Both kernels: 64 slots of up to 8191 keys 65 us, 3.7 TB/s of cache; 4 slots of up to 131072 keys 118 us,
-// 4.1 TB/s, 0.64 of the measured copy bandwidth.  Work is one list of 64-key tiles over (slot, KV head), cut into equal contiguous
+// it the issue slots (60 % busy with three warps per scheduler, ALU 47 %; a fourth warp, at 128 registers, changed nothing): of the
+// 310 warp instructions per 16 keys 120 unpack (48 for K, 72 for V), the rest are parameters, weights, maxima, products and parts,
+// and with four query rows a KV head half of the lanes' weights are padding.  Both kernels: 64 slots of up to 8191 keys 65 us, 3.7 TB/s
+// of cache; 4 slots of up to 131072 keys 118 us, 4.1 TB/s, 0.64 of the measured copy bandwidth.  Work is one list of 64-key tiles over (slot, KV head), cut into equal contiguous
 // ranges, one per warp: a warp streams its tiles by bulk copies through a ring of its own (no barrier between warps) and keeps
 // the online softmax in registers.  Lengths are read on the device, so any raggedness is balanced to a tile.  A range that
 // holds only part of an item leaves (m, l, O) in the workspace and a second kernel (a programmatic dependent) merges the parts
@@ -566,9 +567,11 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && NG < 4 ? 3 : 2) kv4_
         const uint4 w = r < rows ? *reinterpret_cast<const uint4 *>(q + b * 32) : make_uint4(0, 0, 0, 0);
         qb[t][b][0] = w.x, qb[t][b][1] = w.y, qb[t][b][2] = w.z, qb[t][b][3] = w.w;
       }
-      // To fp16, divided by the power of two of the row's largest value: bf16's 8 bits fit fp16's 11, and fp16 keeps its own (small
-      // rows too, of which a sixteenth would be subnormal); values 2^-14 of the largest and less keep 2^-25 of it, a sixteenth of
-      // them 2^-21.  A row of zeros, or with an infinity or a NaN, is converted as it is.
+      // To fp16, the row's largest value brought to its power of two, fp16 rows to 2^4 (bf16 keys may be 2^112 times larger, and their
+      // products are fp32): bf16's 8 bits fit fp16's 11, and fp16 keeps its own (small rows too, of which a sixteenth would be
+      // subnormal); values 2^-14 of that and less keep 2^-25 of it, a sixteenth of them 2^-21.  A row of zeros, or with an infinity
+      // or a NaN, is converted as it is.
+      constexpr int kTop = F16 ? 4 : 0;
       uint32_t most = 0;
 #pragma unroll
       for (int b = 0; b < kWordsK; ++b)
@@ -577,8 +580,8 @@ __global__ void __launch_bounds__(kKvWarps * 32, NT == 1 && NG < 4 ? 3 : 2) kv4_
       most = max(most & 0xffffu, most >> 16);
       most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
       most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
-      const int top = int(__float_as_uint(to_f32<F16>(most)) >> 23), e = top == 0 || top == 255 ? 0 : min(top - 127, 126);
-      const float down = __uint_as_float(uint32_t(127 - e) << 23);
+      const int top = int(__float_as_uint(to_f32<F16>(most)) >> 23), e = top == 0 || top == 255 ? kTop : min(top - 127, 126);
+      const float down = __uint_as_float(uint32_t(127 + kTop - e) << 23);
       back = g.sl / down;
 #pragma unroll
       for (int b = 0; b < kWordsK; ++b)
