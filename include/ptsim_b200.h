@@ -314,7 +314,8 @@ typedef struct ptsim_itab_params {
  * no key gives zeros.  Keys a query does not see never reach its result, whatever they hold.  Rows of o outside every
  * sequence keep their values.  Element (token t, head h, d) of x lies at x_off + t x_row + h x_head + d of argument
  * x_arg (q, k, v may be parts of one argument); offsets and strides are multiples of 8 elements.  A table that
- * descends or leaves the tokens records PTSIM_E_OOB and its sequence is skipped.  bf16 or fp16 throughout; dim 64 or
+ * descends or leaves the tokens records PTSIM_E_OOB and its sequence is skipped (others that overlap on account of it
+ * may be left in part).  bf16 or fp16 throughout; dim 64 or
  * 128; scale > 0, scores scale q.k below 2^20; at most PTSIM_PACKED_SEQS sequences.  One partition unit. */
 #define PTSIM_PACKED_SEQS 1024
 typedef struct ptsim_pattn_params {

@@ -25,7 +25,8 @@
 // Bound: the tensor core, 4 D flop per (query, key, head), and the exponential unit beside it (16384 exponentials of a score
 // tile take as many clocks as its two products at D 128).  One prompt of 8192, 32 / 8 heads of 128: 532 us between idle gaps
 // (1.03 PFLOP/s, 0.60 of the measured burst), 577 back to back under the power cap.  16 prompts of up to 1021: 115 us; each
-// tile costs a chain of softmax, P V and next scores, and each item a set-up, first loads and an epilogue.
+// tile costs a chain of softmax, P V and next scores, and each item a set-up, first loads and an epilogue.  The register split leaves
+// spills (at D 128 200 bytes of loads for T = 1, 372 for T = 2; 144 and 336 at D 64; the one-length kernel has none).
 // P is rounded to the inputs' 16-bit type for the tensor core (half a step, 2^-9 of each weight for bf16, 2^-12 for fp16),
 // as the prefill program does; z, m, l and O are fp32.
 #pragma once
@@ -561,7 +562,9 @@ static int run_packed(const PackedArgs &g, const LaunchCtx &c) {
 // Tiles of a CTA, by the average number of keys of a sequence (the lengths themselves are on the device).  Time of 148 heads
 // (us) with one and with two tiles, dim 128, sequences of n: 64 3.97 / 6.76, 128 5.24 / 7.55, 256 11.0 / 12.8, 512 26.6 / 26.9,
 // 1024 73.7 / 68.6; 256 queries behind 2048 keys 44.9 / 40.7.  Dim 64 (half the products, as many exponentials): 128 3.84 /
-// 5.89, 512 20.7 / 23.8, 1024 57.1 / 60.9, 2048 176 / 180; 256 queries behind 4096 keys 67.6 / 66.8.
+// 5.89, 512 20.7 / 23.8, 1024 57.1 / 60.9, 2048 176 / 180; 256 queries behind 4096 keys 67.6 / 66.8.  All of them batches of one
+// length; of a skewed one (a long prompt beside many short ones, empty sequences, rows of no sequence) the average says little, and
+// neither form has been measured on it.
 static int packed_tiles(const PackedArgs &g, int dim) {
   return int64_t(g.k_tokens) < int64_t(g.seqs) * (dim == 64 ? 4096 : 768) ? 1 : 2;
 }

@@ -2,7 +2,9 @@
 buffers -- what PyTorchSim does when it runs a model's kernels one after another (the bundle's
 manifest.json lists a workload's launches in order, e.g. validation/pytorchsim/
 qwen3_8b_layer_prefill_2048x2048_bf16/manifest.json).  Buffers are allocated once and stay resident;
-a graph can be captured into a CUDA graph so a many-launch workload costs one launch from the host."""
+a graph can be captured into a CUDA graph so a many-launch workload costs one launch from the host.  Buffers
+and workspaces belong to the stream that is current when they are made; a run on another one waits for it first,
+which is the caller's part."""
 import math
 
 from ..codegen import descriptors as D
