@@ -9,7 +9,7 @@
 // of tables that forks share, is a second kernel over the whole GPU (pages_apply_kernel, a programmatic dependent): a warp per
 // 2 KB of a page, four 16-byte loads in flight a lane; its bound is HBM, each moved byte read and written once.  32 forks: 18 us
 // for free, plan and copy (14 captured); 56 MB moved by a compaction between a free and a grow: 23 us for the four kernels,
-// of which the copy's bytes are 9.
+// of which the copy is 14 (its bytes take 9).
 #pragma once
 #include "common.cuh"
 

@@ -93,7 +93,7 @@ def launch_tensors(blob, tensors, lo=0, hi=None, stream=None, sync=True):
     """Run units [lo, hi) of descriptor `blob` over CUDA tensors (argument order), on `stream` (torch's
     current stream by default).  Tensors are used in place.  With sync=True, waits and checks the device
     status word; with sync=False the launch can be captured into a CUDA graph once its device has run one.  The word is the
-    device's and keeps the first failure until it is read: what a launch with sync=False recorded is raised by the next
+    device's and keeps the first failure until it is read (or native.init clears it): what a launch with sync=False recorded is raised by the next
     synchronisation, here, in Graph.run(sync=True) or in native.sync, whichever launch that one follows."""
     torch = _torch()
     desc = D.from_bytes(blob)
