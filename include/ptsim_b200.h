@@ -373,7 +373,8 @@ typedef struct ptsim_kv4_params {
  * counted, copied or moved.
  * The halt word (int32 [1]; halt_arg_p1: 1 + its argument, 0 when absent) ties launches that follow one another without a ptsim_sync: a GROW,
  * FORK or COPY that is refused sets it to its code, and every PAGES and KV4_STORE launch that has it and finds it nonzero
- * changes nothing.  The cache stays as it was before the refused launch until the caller clears the word.  One partition unit. */
+ * changes nothing and records that code.  The cache stays as it was before the refused launch until the caller clears the word.
+ * One partition unit. */
 #define PTSIM_PAGES_GROW 1
 #define PTSIM_PAGES_FORK 2
 #define PTSIM_PAGES_COPY 3

@@ -32,6 +32,7 @@
 #include "sm100.cuh"
 #include "decode.cuh"
 #include "packed.cuh"
+#include "pages.cuh"
 
 namespace ptsim {
 
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(256) kv4_store_kernel(const __grid_constant__ 
   const uint32_t t = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int h0 = int(blockIdx.y) * (kHeads * HS) + lane / kLanes;
   pdl_enter();
-  if (t >= uint32_t(g.tokens) || (g.halt != nullptr && *g.halt != 0)) return;
+  if (halted(g.halt) || t >= uint32_t(g.tokens)) return;
   const Kv4Lane<D, NG> me(lane);
   const uint16_t *src = me.is_v ? g.b + t * g.b_row : g.a + t * g.a_row;
   const int64_t step_h = me.is_v ? g.b_head : g.a_head;

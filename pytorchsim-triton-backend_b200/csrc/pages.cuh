@@ -28,7 +28,13 @@ struct PagesArgs {
   int32_t op, n, slots, pages, page_size, max_pages, layers;
 };
 
-__device__ __forceinline__ bool pages_halted(const PagesArgs &g) { return g.halt != nullptr && *g.halt != 0; }
+// Does the halt word (null: none) stop this launch?  Every launch that it stops records why, so a synchronisation after any of them
+// fails.
+__device__ __forceinline__ bool halted(const int32_t *halt) {
+  const int why = halt == nullptr ? 0 : *halt;
+  if (why != 0 && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) record_status(why);
+  return why != 0;
+}
 __device__ __forceinline__ int pages_held(const PagesArgs &g, int len) { return (len + g.page_size - 1) / g.page_size; }
 __device__ __forceinline__ bool pages_len_ok(const PagesArgs &g, int len) {
   return len >= 0 && len <= int64_t(g.max_pages) * g.page_size;
@@ -74,7 +80,7 @@ __global__ void __launch_bounds__(kPagesThreads) pages_plan_kernel(const __grid_
   const int i = threadIdx.x;
   if (i == 0) refused = 0, asked = 0;
   pdl_enter();
-  if (pages_halted(g)) {
+  if (halted(g.halt)) {
     if (i == 0) g.head[0] = -1;
     return;
   }
@@ -268,7 +274,7 @@ __global__ void __launch_bounds__(256) pages_apply_kernel(const __grid_constant_
 // One CTA per listed slot.
 __global__ void __launch_bounds__(256) pages_free_kernel(const __grid_constant__ PagesArgs g) {
   pdl_enter();
-  if (pages_halted(g)) return;
+  if (halted(g.halt)) return;
   const int id = g.ids[blockIdx.x];
   bool again = false;
   for (int j = threadIdx.x; j < int(blockIdx.x); j += 256) again |= g.ids[j] == id;

@@ -961,10 +961,11 @@ def test_a_captured_decode_step_that_runs_out_of_pages_leaves_the_cache():
     assert e.value.code == D.E_RESOURCE and state["halt"].tolist() == [D.E_RESOURCE]
     for t, n in zip(books, ("table", "lens", "refs", "pool")):
         assert torch.equal(t, state[n]), n
-    native.sync(stream)                                      # the halted replays recorded nothing more
     del past[16:]
-    launch(B.pages_free(c, 1, halt=True), [ints([3])] + [state[n] for n in ("table", "lens", "refs", "halt")])
-    assert state["lens"].tolist() == [16] * 4                # halted as well
+    for desc, ts in ((B.pages_free(c, 1, halt=True), [ints([3])] + [state[n] for n in ("table", "lens", "refs", "halt")]),
+                     (B.kv4_store(c, 4, fused_hq=hq, halt=True), [state[n] for n in ("qkv", "cu", "lens", "table", "pool", "halt")])):
+        assert failed(desc, ts) == D.E_RESOURCE              # halted as well, and each says so
+        assert state["lens"].tolist() == [16] * 4 and torch.equal(books[3], state["pool"])
     launch(B.pages_free(c, 3), [ints([1, 2, 3])] + [state[n] for n in ("table", "lens", "refs")])
     state["halt"].zero_()
     step()
